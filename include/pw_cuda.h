@@ -135,6 +135,7 @@ typedef struct pw_router {
  * src/text_endpoint.rs:5507-5512). */
 #define PW_NORM_F32 0u
 #define PW_NORM_BF16 1u
+#define PW_NORM_F16 2u /* pw_add_rms_norm only */
 
 /* An RMSNorm (reference: rms_norm src/text_endpoint.rs:2939 with
  * stable_rms_inverse src/lib.rs:1890).  Device pointer. */
@@ -144,6 +145,51 @@ typedef struct pw_norm {
   uint32_t weight_dtype; /* PW_NORM_F32 or PW_NORM_BF16 */
   float epsilon;         /* layernorm_epsilon (1e-5 for MiMo-V2.5), finite and > 0 */
 } pw_norm;
+
+/* Element types of the rows that pw_add_rms_norm, pw_linear and
+ * pw_fp8_linear_codes read and write.  F32 here is a full f32 value (the f32
+ * rows of the other calls hold bf16 values: they can be passed as they are). */
+#define PW_DTYPE_F32 0u
+#define PW_DTYPE_BF16 1u
+#define PW_DTYPE_F16 2u
+
+/* Rows of a matrix: row r starts r * stride elements after `data`.  stride is
+ * at least the row length (0 = rows follow one another).  Host or device
+ * memory per the call's `mem`, aligned to the element. */
+typedef struct pw_rows {
+  void *data;
+  uint64_t stride;
+  uint32_t dtype; /* PW_DTYPE_* */
+  uint32_t reserved; /* 0 */
+} pw_rows;
+
+/* A dense 16-bit weight [rows, cols], rows as in pw_rows (the checkpoint's
+ * BF16 o_proj and lm_head; reference: execute_bf16_linear,
+ * kernels/block_fp8_gemv.metal:358).  Device pointer.  Every row starts at a
+ * 16-byte boundary: stride (0 = cols) is a multiple of 8. */
+typedef struct pw_dense {
+  const void *weight;
+  uint64_t stride;
+  uint32_t rows, cols;
+  uint32_t dtype; /* PW_DTYPE_BF16 or PW_DTYPE_F16 */
+  uint32_t reserved; /* 0 */
+} pw_dense;
+
+/* What a linear layer applies to its 32-bit sums before the one rounding to
+ * the output's type: y = activation(sum + bias) + residual. */
+#define PW_ACT_NONE 0u
+#define PW_ACT_RELU 1u
+#define PW_ACT_GELU 2u      /* v (1 + erf(v / sqrt 2)) / 2 */
+#define PW_ACT_GELU_TANH 3u /* v (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) / 2 */
+#define PW_ACT_SILU 4u      /* v / (1 + exp(-v)) */
+typedef struct pw_epilogue {
+  const void *bias;    /* [output columns], device pointer; NULL: none */
+  uint32_t bias_dtype; /* PW_DTYPE_* */
+  uint32_t activation; /* PW_ACT_* */
+  pw_rows residual;    /* [width, output columns], `mem` as the rows; data NULL: none.
+                          May be the output itself (same data, stride and dtype),
+                          otherwise must not overlap it. */
+} pw_epilogue;
 
 /* Per-call accounting (reference: WideMoeExecution / WideLinearExecution,
  * src/wide_metal_moe.rs:97-111). */
@@ -257,6 +303,52 @@ int pw_route(pw_runtime *rt, const pw_router *router, const float *x, uint32_t t
  * PW_ERR_NONFINITE (stable_rms_inverse's Err). */
 int pw_rms_norm(pw_runtime *rt, const pw_norm *norm, const float *x, uint32_t rows, float *y, float *inverse,
                 uint32_t mem, pw_stats *stats);
+
+/* ------------------------------------- residual, norm, linear layers */
+
+/* The residual's addition, an RMSNorm and its 8-bit output in one pass:
+ *   s = round(x + residual)            (x's type; s = x without a residual)
+ *   v = s / sqrt(mean(s^2) + epsilon) * weight            (f32, not rounded)
+ *   y = round(v)                                            (y's type)
+ *   scales[r, g] = max(absmax of v over columns 128 g .. 128 g + 127, 1e-10) / 448
+ *   codes[r, c] = e4m3(v / scales[r, c / 128])        (round to nearest even)
+ * codes u8 [rows, hidden] and scales f32 [rows, ceil(hidden / 128)] are
+ * contiguous: what pw_fp8_linear_codes takes.  Unlike pw_rms_norm, which
+ * reproduces the reference's sum order and its bf16 value between the two
+ * products, this rounds y once and quantizes v itself; hidden is any size up
+ * to 16384 (a multiple of 256 there).
+ * x, residual and sum have one dtype; y has that dtype or F32.  `residual`,
+ * `sum`, `y` and codes + scales (both or neither) are optional (NULL); at least
+ * one of y and codes is asked for.  sum may be x or residual itself, and y may
+ * be x (same data and stride); other overlaps are not allowed.
+ * A row whose s is not finite is PW_ERR_NONFINITE (PW_FLAG_NONFINITE_INPUT);
+ * its outputs are unspecified, other rows are not affected.  A value that
+ * leaves y's range raises PW_FLAG_NONFINITE_ROUND. */
+int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const pw_rows *residual, uint32_t rows,
+                    const pw_rows *sum, const pw_rows *y, uint8_t *codes, float *scales, uint32_t mem,
+                    pw_stats *stats);
+
+/* Linear layer over a 16-bit weight: y = act(x W^T + bias) + residual with
+ * 32-bit sums and one rounding to y's type.  x [width, w->cols] has the
+ * weight's dtype, or F32, which is rounded to the weight's dtype first (exact
+ * for the library's bf16-valued rows over a BF16 weight).  y [width, w->rows]
+ * has any dtype; y may be residual, not x.  Any width, rows and cols >= 1; x
+ * rows that do not start at 16-byte boundaries are copied first.  `ep` may be
+ * NULL.  A non-finite output is PW_ERR_NONFINITE (PW_FLAG_NONFINITE_ROUND).
+ * Results do not depend on the other tokens of the call or, between widths of
+ * one kernel, on the width. */
+int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t width, const pw_epilogue *ep,
+              const pw_rows *y, uint32_t mem, pw_stats *stats);
+
+/* pw_fp8_linear on activations that are already quantized (pw_quantize_fp8,
+ * pw_add_rms_norm), with the epilogue of pw_linear: codes u8 [width, cols] and
+ * scales f32 [width, cols / 128], contiguous, y [width, rows] of any dtype.
+ * The sums are those of pw_fp8_linear (the same kernels), so y of dtype F32
+ * without an epilogue equals its PW_OUTPUT_F32 output bit for bit.  Shapes as
+ * in pw_fp8_linear; codes start at a 16-byte boundary. */
+int pw_fp8_linear_codes(pw_runtime *rt, const pw_fp8_tensor *w, uint32_t layout, const uint8_t *codes,
+                        const float *scales, uint32_t width, const pw_epilogue *ep, const pw_rows *y, uint32_t mem,
+                        pw_stats *stats);
 
 /* ------------------------------------------------------------ MoE layers */
 

@@ -63,6 +63,9 @@ def _bind(L: ctypes.CDLL) -> None:
     L.pw_dense_mlp.argtypes = [vp, vp, vp, u32, vp, u32, vp]
     L.pw_moe_block.argtypes = [vp, vp, vp, vp, vp, u32, vp, vp, vp, u32, vp]
     L.pw_ep_moe_block.argtypes = [vp, vp, vp, vp, vp, u32, vp, vp, vp, u32, vp]
+    L.pw_add_rms_norm.argtypes = [vp, vp, vp, vp, u32, vp, vp, vp, vp, u32, vp]
+    L.pw_linear.argtypes = [vp, vp, vp, u32, vp, vp, u32, vp]
+    L.pw_fp8_linear_codes.argtypes = [vp, vp, u32, vp, vp, u32, vp, vp, u32, vp]
     L.pw_set_profiling.argtypes = [vp, i32]
     L.pw_last_profile.argtypes = [vp, vp]
     for name in header_symbols():

@@ -45,6 +45,17 @@ cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+// A linear layer's epilogue and output rows (device pointers; pw_epilogue.cuh):
+// y[t, c] = round(act(sum + bias[c]) + residual[t, c]).
+struct EpilogueArgs {
+  const void *bias;      // nullptr: none
+  const void *residual;  // nullptr: none; may be y
+  void *y;
+  uint64_t residual_stride, y_stride;  // elements between rows
+  uint32_t bias_dtype, residual_dtype, y_dtype;  // PW_DTYPE_*
+  uint32_t act;                                  // PW_ACT_*
+};
+
 // One group of tokens sharing one weight matrix (a projection call, or one
 // expert's placements in a routed layer).  count <= 8 per group: wider token
 // sets are split into several groups over the same weights.
@@ -96,6 +107,7 @@ struct GemvArgs {
   const GemvGroup *l2_next;      // optional: the next kernel's groups (same count); CTAs with
   uint32_t l2_rows, l2_cols;     //   no unit of their own prefetch those groups' w0 [rows, cols]
                                  //   into L2 while the others stream
+  EpilogueArgs ep;               // kind 4: bias, activation, residual and the output rows
 };
 
 // Wide-width grouped GEMM (tcgen05): the GEMV arguments plus TMA maps of the
@@ -122,7 +134,8 @@ cudaError_t launch_quantize(const float *x, uint32_t rows, uint32_t cols, uint8_
                             uint32_t *zero = nullptr, uint32_t n_zero = 0);
 // kind: 0 = block-scaled (quantized x) over each group's w0/s0, 1 = readable
 // (f32 x), 2 = fused gate/up SwiGLU over w0/s0 and w1/s1, 3 = block-scaled
-// over w1/s1 (the unfused up projection)
+// over w1/s1 (the unfused up projection), 4 = kind 0 with the epilogue `ep`
+// (pw_epilogue.cuh) instead of `out` / `round_bf16`
 cudaError_t launch_gemv(int kind, const GemvArgs &args, int grid, cudaStream_t stream);
 int gemv_max_ctas(int num_sms);
 cudaError_t launch_gemv_mma(int kind, const GemvArgs &args, int grid, cudaStream_t stream);
@@ -217,6 +230,41 @@ cudaError_t launch_swiglu(const float *gate, const float *up, float *h, uint32_t
                           cudaStream_t stream, const uint32_t *rows_dev = nullptr, uint32_t row_len = 1);
 cudaError_t launch_validate_fp8(const uint8_t *w, uint64_t n, const float *s, uint64_t ns,
                                 unsigned long long *first_bad, uint32_t *flags, cudaStream_t stream);
+
+// The residual's addition, RMSNorm and FP8 output in one pass (pw_add_norm.cu).
+struct AddNormArgs {
+  const void *x, *residual;  // residual: nullptr for none
+  void *sum, *y;             // optional
+  uint8_t *codes;            // optional, with scales
+  float *scales;
+  const void *weight;
+  uint64_t x_stride, residual_stride, sum_stride, y_stride;  // elements
+  uint32_t rows, hidden;
+  uint32_t dtype, y_dtype, w_dtype;  // PW_DTYPE_*, PW_DTYPE_*, PW_NORM_*
+  float eps;
+  uint32_t *flags;
+};
+cudaError_t launch_add_norm(const AddNormArgs &a, int num_sms, cudaStream_t stream);
+
+// 16-bit linear layer (pw_linear.cu): ep.y[t, r] from x [width, cols] and w
+// [rows, cols], both of `dtype` (BF16 or F16), rows 16-byte aligned.
+struct LinearArgs {
+  const void *x, *w;
+  uint64_t x_stride, w_stride;  // elements
+  uint32_t width, rows, cols, dtype;
+  EpilogueArgs ep;
+  uint32_t *flags;
+};
+cudaError_t launch_linear(const LinearArgs &a, int num_sms, cudaStream_t stream);
+// out[r, c] (rows of `out_stride` elements of 16-bit dtype) = x[r, c]
+// converted from x_dtype.
+cudaError_t launch_convert_rows(const void *x, uint64_t x_stride, uint32_t x_dtype, uint32_t rows, uint32_t cols,
+                                void *out, uint64_t out_stride, uint32_t dtype, cudaStream_t stream);
+// cuTensorMapEncodeTiled over 16-bit rows: with k_blocks, the view {64
+// columns, rows, cols / 64} in boxes {64, box_rows, k_blocks}; without, the
+// view {cols, rows, 1} in boxes {64, box_rows, 1}, zero past the last column.
+bool encode_rows16_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride,
+                       uint32_t dtype, uint32_t box_rows, uint32_t k_blocks);
 
 // Expert-parallel window of one rank (byte offsets from its base): flags
 // written by peers (ready for an epoch, data sent, rows returned), the

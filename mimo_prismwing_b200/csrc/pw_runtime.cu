@@ -66,6 +66,21 @@ bool encode_act_maps(CUtensorMap (&out)[4], const void *base, uint32_t rows, uin
   return true;
 }
 
+// 16-bit rows for the linear layer's TMA loads (zero past every end).
+bool encode_rows16_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride,
+                       uint32_t dtype, uint32_t box_rows, uint32_t k_blocks) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn || rows == 0 || cols == 0 || stride % 8u || (k_blocks && cols % 64u)) return false;
+  cuuint64_t dims[3] = {k_blocks ? 64u : cols, rows, k_blocks ? cols / 64u : 1u};
+  cuuint64_t strides[2] = {stride * 2u, k_blocks ? 128u : stride * 2u};
+  cuuint32_t box[3] = {64u, box_rows, k_blocks ? k_blocks : 1u};
+  cuuint32_t estr[3] = {1u, 1u, 1u};
+  return fn(out, dtype == PW_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // The weight is viewed as {128 B, rows, k-blocks} with strides {cols, 128}:
 // a box of {128, box_rows, 256 / box_rows} is 32 KB and lands row-major in
 // shared memory (one 128-byte line per row and k-block), 128B-swizzled.
@@ -863,6 +878,382 @@ int pw_fp8_gemv(pw_runtime *rt, const pw_fp8_tensor *w, const float *x, uint32_t
 int pw_fp8_linear(pw_runtime *rt, const pw_fp8_tensor *w, uint32_t layout, const float *x, uint32_t width, float *y,
                   uint32_t mem, pw_stats *stats) {
   return projection(rt, (layout & PW_OUTPUT_F32) ? 4 : 0, w, layout & ~PW_OUTPUT_F32, x, width, y, mem, stats);
+}
+
+}  // extern "C"
+
+// -------------------------------------- residual, norm, linear layers
+namespace {
+
+// The caller's device comes back when the call ends.
+struct DeviceScope {
+  int before = -1;
+  cudaError_t enter(int device) {
+    cudaError_t e = cudaGetDevice(&before);
+    if (e != cudaSuccess) before = -1;
+    if (e == cudaSuccess && before != device) return cudaSetDevice(device);
+    before = -1;
+    return e;
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+size_t elem_size(uint32_t dtype) { return dtype == PW_DTYPE_F32 ? 4u : 2u; }
+
+// Checks a caller's rows of `len` elements and fills in stride 0.
+int check_rows(pw_runtime *rt, const char *name, const pw_rows *in, uint32_t rows, uint64_t len, pw_rows &out) {
+  if (!in || !in->data) return fail(rt, PW_ERR_ARGUMENT, "%s is null", name);
+  out = *in;
+  if (out.dtype > PW_DTYPE_F16 || out.reserved != 0u) return fail(rt, PW_ERR_ARGUMENT, "%s: unknown dtype", name);
+  if (out.stride == 0u) out.stride = len;
+  if (out.stride < len) return fail(rt, PW_ERR_SHAPE, "%s: row stride below the row length", name);
+  if (rows == 1u) out.stride = (len + 7u) & ~(uint64_t)7u;  // one row has no stride to keep
+  if (out.stride > ((uint64_t)1 << 40) || (uint64_t)rows * out.stride > ((uint64_t)1 << 48))
+    return fail(rt, PW_ERR_SHAPE, "%s: row stride out of range", name);
+  if (reinterpret_cast<uintptr_t>(out.data) % elem_size(out.dtype))
+    return fail(rt, PW_ERR_ARGUMENT, "%s is not aligned to its elements", name);
+  return PW_OK;
+}
+
+struct Span {
+  uintptr_t at;
+  uint64_t row, stride, rows;  // bytes
+};
+Span span(const pw_rows &m, uint32_t rows, uint64_t len) {
+  const uint64_t z = elem_size(m.dtype);
+  return {reinterpret_cast<uintptr_t>(m.data), len * z, m.stride * z, rows};
+}
+bool same(const pw_rows &a, const pw_rows &b) { return a.data == b.data && a.stride == b.stride && a.dtype == b.dtype; }
+// Whether two sets of rows share memory; columns of one wider buffer do not.
+bool overlap(const Span &a, const Span &b) {
+  const uintptr_t a_end = a.at + (a.rows - 1u) * a.stride + a.row, b_end = b.at + (b.rows - 1u) * b.stride + b.row;
+  if (a_end <= b.at || b_end <= a.at) return false;
+  if (a.stride != b.stride) return true;
+  const uint64_t d = a.at <= b.at ? (b.at - a.at) % a.stride : (a.stride - (a.at - b.at) % a.stride) % a.stride;
+  return d < a.row || d + b.row > a.stride;
+}
+
+// Device rows of a host call: packed, each row start 16-byte aligned.
+pw_rows device_rows(Arena &ar, const pw_rows &m, uint32_t rows, uint64_t len) {
+  pw_rows d = m;
+  d.stride = (len + 7u) & ~(uint64_t)7u;
+  d.data = ar.take<uint8_t>((size_t)rows * d.stride * elem_size(m.dtype));
+  return d;
+}
+cudaError_t copy_rows(const pw_rows &to, const pw_rows &from, uint32_t rows, uint64_t len, cudaMemcpyKind kind,
+                      cudaStream_t stream) {
+  const size_t z = elem_size(to.dtype);
+  return cudaMemcpy2DAsync(to.data, to.stride * z, from.data, from.stride * z, len * z, rows, kind, stream);
+}
+
+// Checks an epilogue and its output rows and turns them into kernel arguments;
+// with the residual's and y's caller rows in `res` and `out`.
+int check_epilogue(pw_runtime *rt, const pw_epilogue *ep, const pw_rows *y, uint32_t width, uint32_t cols,
+                   EpilogueArgs &e, pw_rows &res, pw_rows &out) {
+  int s;
+  if ((s = check_rows(rt, "y", y, width, cols, out)) != PW_OK) return s;
+  e = EpilogueArgs{};
+  res = pw_rows{};
+  if (ep) {
+    if (ep->activation > PW_ACT_SILU) return fail(rt, PW_ERR_ARGUMENT, "unknown activation %u", ep->activation);
+    if (ep->bias_dtype > PW_DTYPE_F16) return fail(rt, PW_ERR_ARGUMENT, "bias: unknown dtype");
+    if (ep->bias && reinterpret_cast<uintptr_t>(ep->bias) % elem_size(ep->bias_dtype))
+      return fail(rt, PW_ERR_ARGUMENT, "bias is not aligned to its elements");
+    e.bias = ep->bias;
+    e.bias_dtype = ep->bias_dtype;
+    e.act = ep->activation;
+    if (ep->residual.data) {
+      if ((s = check_rows(rt, "residual", &ep->residual, width, cols, res)) != PW_OK) return s;
+      if (!same(res, out) && overlap(span(res, width, cols), span(out, width, cols)))
+        return fail(rt, PW_ERR_ARGUMENT, "residual overlaps y without being y");
+    }
+  }
+  return PW_OK;
+}
+
+void set_rows(EpilogueArgs &e, const pw_rows &res, const pw_rows &out) {
+  e.residual = res.data;
+  e.residual_stride = res.stride;
+  e.residual_dtype = res.dtype;
+  e.y = out.data;
+  e.y_stride = out.stride;
+  e.y_dtype = out.dtype;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const pw_rows *residual, uint32_t rows,
+                    const pw_rows *sum, const pw_rows *y, uint8_t *codes, float *scales, uint32_t mem,
+                    pw_stats *stats) {
+  if (!rt) return PW_ERR_ARGUMENT;
+  if (!norm || !norm->weight) return fail(rt, PW_ERR_ARGUMENT, "norm descriptor is null");
+  if (norm->weight_dtype > PW_NORM_F16) return fail(rt, PW_ERR_ARGUMENT, "unknown norm weight_dtype");
+  if (!std::isfinite(norm->epsilon) || norm->epsilon <= 0.0f) return fail(rt, PW_ERR_ARGUMENT, "invalid RMSNorm epsilon");
+  const uint32_t H = norm->hidden;
+  if (H == 0 || H > 16384u) return fail(rt, PW_ERR_SHAPE, "RMSNorm shape mismatch (hidden %u, 1 to 16384)", H);
+  if (rows == 0) return fail(rt, PW_ERR_SHAPE, "RMSNorm needs at least one row");
+  if (!codes != !scales) return fail(rt, PW_ERR_ARGUMENT, "codes and scales go together");
+  if (!y && !codes) return fail(rt, PW_ERR_ARGUMENT, "nothing asked for: neither y nor codes");
+  if (reinterpret_cast<uintptr_t>(scales) % 4u) return fail(rt, PW_ERR_ARGUMENT, "scales are not aligned to their elements");
+  int s;
+  pw_rows xr{}, rr{}, sr{}, yr{};
+  if ((s = check_rows(rt, "x", x, rows, H, xr)) != PW_OK) return s;
+  if (residual && (s = check_rows(rt, "residual", residual, rows, H, rr)) != PW_OK) return s;
+  if (sum && (s = check_rows(rt, "sum", sum, rows, H, sr)) != PW_OK) return s;
+  if (y && (s = check_rows(rt, "y", y, rows, H, yr)) != PW_OK) return s;
+  if ((residual && rr.dtype != xr.dtype) || (sum && sr.dtype != xr.dtype))
+    return fail(rt, PW_ERR_ARGUMENT, "x, residual and sum must have one dtype");
+  if (y && yr.dtype != xr.dtype && yr.dtype != PW_DTYPE_F32)
+    return fail(rt, PW_ERR_ARGUMENT, "y must have x's dtype or F32");
+  const uint64_t G = (H + 127u) / 128u;
+  // every output apart from the others and from the inputs, but for the
+  // in-place forms: a thread reads all it needs of a row before it writes
+  const Span outs[4] = {span(sr, rows, H), span(yr, rows, H), {reinterpret_cast<uintptr_t>(codes), H, H, rows},
+                        {reinterpret_cast<uintptr_t>(scales), G * 4u, G * 4u, rows}};
+  const bool has[4] = {sum != nullptr, y != nullptr, codes != nullptr, codes != nullptr};
+  for (int i = 0; i < 4; ++i) {
+    if (!has[i]) continue;
+    for (int j = i + 1; j < 4; ++j)
+      if (has[j] && overlap(outs[i], outs[j])) return fail(rt, PW_ERR_ARGUMENT, "outputs overlap");
+    const bool as_x = (i == 0 && same(sr, xr)) || (i == 1 && same(yr, xr));
+    const bool as_r = i == 0 && residual && same(sr, rr);
+    if (!as_x && overlap(outs[i], span(xr, rows, H))) return fail(rt, PW_ERR_ARGUMENT, "an output overlaps x");
+    if (residual && !as_r && overlap(outs[i], span(rr, rows, H)))
+      return fail(rt, PW_ERR_ARGUMENT, "an output overlaps residual");
+  }
+  DeviceScope dev;
+  CK(dev.enter(rt->device));
+  Call call{rt, mem, stats, 0};
+  if ((s = call.begin()) != PW_OK) return s;
+  Arena ar;
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1) {
+      if (ar.off && (s = ensure_scratch(rt, ar.off)) != PW_OK) return s;
+      ar = Arena{static_cast<char *>(rt->scratch), 0};
+    }
+    pw_rows dx = xr, dr = rr, ds = sr, dy = yr;
+    uint8_t *dc = codes;
+    float *dsc = scales;
+    if (call.host()) {
+      dx = device_rows(ar, xr, rows, H);
+      if (residual) dr = device_rows(ar, rr, rows, H);
+      if (sum) ds = device_rows(ar, sr, rows, H);
+      if (y) dy = device_rows(ar, yr, rows, H);
+      if (codes) {
+        dc = ar.take<uint8_t>((size_t)rows * H);
+        dsc = ar.take<float>((size_t)rows * G);
+      }
+    }
+    if (pass == 0) continue;
+    if (call.host()) {
+      CK(copy_rows(dx, xr, rows, H, cudaMemcpyHostToDevice, rt->stream));
+      if (residual) CK(copy_rows(dr, rr, rows, H, cudaMemcpyHostToDevice, rt->stream));
+    }
+    AddNormArgs a{};
+    a.x = dx.data;
+    a.residual = dr.data;
+    a.sum = ds.data;
+    a.y = dy.data;
+    a.codes = dc;
+    a.scales = dsc;
+    a.weight = norm->weight;
+    a.x_stride = dx.stride;
+    a.residual_stride = dr.stride;
+    a.sum_stride = ds.stride;
+    a.y_stride = dy.stride;
+    a.rows = rows;
+    a.hidden = H;
+    a.dtype = xr.dtype;
+    a.y_dtype = y ? yr.dtype : xr.dtype;
+    a.w_dtype = norm->weight_dtype;
+    a.eps = norm->epsilon;
+    a.flags = rt->d_flags;
+    {
+      ProfScope ps(rt, P_QUANT, 1);
+      CK(launch_add_norm(a, rt->num_sms, rt->stream));
+    }
+    if (call.host()) {
+      if (sum) CK(copy_rows(sr, ds, rows, H, cudaMemcpyDeviceToHost, rt->stream));
+      if (y) CK(copy_rows(yr, dy, rows, H, cudaMemcpyDeviceToHost, rt->stream));
+      if (codes) {
+        if ((s = call.stage_out(codes, dc, (size_t)rows * H)) != PW_OK) return s;
+        if ((s = call.stage_out(scales, dsc, (size_t)rows * G * 4u)) != PW_OK) return s;
+      }
+    }
+  }
+  return call.finish((uint64_t)H * (norm->weight_dtype == PW_NORM_F32 ? 4u : 2u));
+}
+
+int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t width, const pw_epilogue *ep,
+              const pw_rows *y, uint32_t mem, pw_stats *stats) {
+  if (!rt) return PW_ERR_ARGUMENT;
+  if (!w || !w->weight) return fail(rt, PW_ERR_ARGUMENT, "weight descriptor is null");
+  if ((w->dtype != PW_DTYPE_BF16 && w->dtype != PW_DTYPE_F16) || w->reserved != 0u)
+    return fail(rt, PW_ERR_ARGUMENT, "weight dtype must be PW_DTYPE_BF16 or PW_DTYPE_F16");
+  if (w->rows == 0 || w->cols == 0) return fail(rt, PW_ERR_SHAPE, "linear weight is empty");
+  if (w->rows > (1u << 30) || w->cols > (1u << 30)) return fail(rt, PW_ERR_UNSUPPORTED, "linear weight too large");
+  if (width == 0) return fail(rt, PW_ERR_SHAPE, "linear layer needs at least one row");
+  if (width > (1u << 30)) return fail(rt, PW_ERR_UNSUPPORTED, "too many rows");
+  const uint32_t K = w->cols, N = w->rows;
+  uint64_t ws = w->stride ? w->stride : K;
+  if (N == 1u) ws = ((uint64_t)K + 7u) & ~(uint64_t)7u;
+  if (ws < K) return fail(rt, PW_ERR_SHAPE, "weight row stride below its columns");
+  if (reinterpret_cast<uintptr_t>(w->weight) % 16u || ws % 8u || ws >= ((uint64_t)1 << 36))
+    return fail(rt, PW_ERR_UNSUPPORTED, "weight rows must start at 16-byte boundaries (stride a multiple of 8)");
+  int s;
+  pw_rows xr{}, rr{}, yr{};
+  EpilogueArgs e{};
+  if ((s = check_rows(rt, "x", x, width, K, xr)) != PW_OK) return s;
+  if (xr.dtype != w->dtype && xr.dtype != PW_DTYPE_F32)
+    return fail(rt, PW_ERR_ARGUMENT, "x must have the weight's dtype or F32");
+  if ((s = check_epilogue(rt, ep, y, width, N, e, rr, yr)) != PW_OK) return s;
+  if (overlap(span(xr, width, K), span(yr, width, N))) return fail(rt, PW_ERR_ARGUMENT, "y overlaps x");
+  DeviceScope dev;
+  CK(dev.enter(rt->device));
+  Call call{rt, mem, stats, 0};
+  if ((s = call.begin()) != PW_OK) return s;
+  Arena ar;
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1) {
+      if (ar.off && (s = ensure_scratch(rt, ar.off)) != PW_OK) return s;
+      ar = Arena{static_cast<char *>(rt->scratch), 0};
+    }
+    pw_rows dx = xr, dr = rr, dy = yr;
+    if (call.host()) {
+      dx = device_rows(ar, xr, width, K);
+      if (rr.data) dr = device_rows(ar, rr, width, N);
+      dy = device_rows(ar, yr, width, N);
+    }
+    // TMA reads rows that start at 16-byte boundaries, of the weight's type
+    const bool convert = xr.dtype != w->dtype || (!call.host() && (reinterpret_cast<uintptr_t>(xr.data) % 16u ||
+                                                                   xr.stride % 8u || xr.stride >= ((uint64_t)1 << 36)));
+    pw_rows cx = dx;
+    if (convert) {
+      cx.dtype = w->dtype;
+      cx = device_rows(ar, cx, width, K);
+    }
+    if (pass == 0) continue;
+    if (call.host()) {
+      CK(copy_rows(dx, xr, width, K, cudaMemcpyHostToDevice, rt->stream));
+      if (rr.data) CK(copy_rows(dr, rr, width, N, cudaMemcpyHostToDevice, rt->stream));
+    }
+    if (convert) {
+      ProfScope ps(rt, P_QUANT, 1);
+      CK(launch_convert_rows(dx.data, dx.stride, dx.dtype, width, K, cx.data, cx.stride, cx.dtype, rt->stream));
+    }
+    LinearArgs a{};
+    a.x = cx.data;
+    a.w = w->weight;
+    a.x_stride = cx.stride;
+    a.w_stride = ws;
+    a.width = width;
+    a.rows = N;
+    a.cols = K;
+    a.dtype = w->dtype;
+    a.ep = e;
+    set_rows(a.ep, dr, dy);
+    a.flags = rt->d_flags;
+    {
+      ProfScope ps(rt, P_PROJ, 1);
+      CK(launch_linear(a, rt->num_sms, rt->stream));
+    }
+    if (call.host()) CK(copy_rows(yr, dy, width, N, cudaMemcpyDeviceToHost, rt->stream));
+  }
+  return call.finish((uint64_t)N * K * 2u);
+}
+
+int pw_fp8_linear_codes(pw_runtime *rt, const pw_fp8_tensor *w, uint32_t layout, const uint8_t *codes,
+                        const float *scales, uint32_t width, const pw_epilogue *ep, const pw_rows *y, uint32_t mem,
+                        pw_stats *stats) {
+  if (!rt) return PW_ERR_ARGUMENT;
+  if (width == 0) return fail(rt, PW_ERR_SHAPE, "wide row count must be at least one");
+  if (!codes || !scales) return fail(rt, PW_ERR_ARGUMENT, "null activation pointer");
+  int s;
+  if ((s = check_projection(rt, w, layout)) != PW_OK) return s;
+  if (width > (1u << 30)) return fail(rt, PW_ERR_UNSUPPORTED, "too many rows");
+  if (reinterpret_cast<uintptr_t>(scales) % 4u) return fail(rt, PW_ERR_ARGUMENT, "scales are not aligned to their elements");
+  const bool host = (mem & PW_MEM_HOST) != 0;
+  if (!host && reinterpret_cast<uintptr_t>(codes) % 16u)
+    return fail(rt, PW_ERR_UNSUPPORTED, "activation codes must start at a 16-byte boundary");
+  const uint32_t K = w->cols, N = w->rows;
+  pw_rows rr{}, yr{};
+  EpilogueArgs e{};
+  if ((s = check_epilogue(rt, ep, y, width, N, e, rr, yr)) != PW_OK) return s;
+  const Span in_codes{reinterpret_cast<uintptr_t>(codes), K, K, width};
+  const Span in_scales{reinterpret_cast<uintptr_t>(scales), K / 128u * 4u, K / 128u * 4u, width};
+  if (overlap(span(yr, width, N), in_codes) || overlap(span(yr, width, N), in_scales))
+    return fail(rt, PW_ERR_ARGUMENT, "y overlaps the activations");
+  DeviceScope dev;
+  CK(dev.enter(rt->device));
+  // Device-resident map and groups of each piece of the batch (a piece's
+  // records fill one descriptor slot), built on the first call of a shape.
+  constexpr uint32_t kPiece = 6144;
+  const bool wide = width >= kWideProjection;
+  const uint32_t chunk = wide ? (uint32_t)gemm_tc_tokens(4) : 8u;
+  const uint32_t box_rows = wide && layout != PW_LAYOUT_PLAIN ? 64u : map_box_rows(layout);
+  const uint32_t box_kb = wide && layout != PW_LAYOUT_PLAIN ? 1u : 0u;
+  Call call{rt, mem, stats, 0};
+  if ((s = call.begin()) != PW_OK) return s;
+  const bool chain = !wide && !rt->profiling;
+  PdlScope pdl(chain);
+  Arena ar;
+  for (int pass = 0; pass < 2; ++pass) {
+    if (pass == 1) {
+      if (ar.off && (s = ensure_scratch(rt, ar.off)) != PW_OK) return s;
+      ar = Arena{static_cast<char *>(rt->scratch), 0};
+    }
+    const size_t nx = (size_t)width * K;
+    const uint8_t *dc = codes;
+    const float *dsc = scales;
+    pw_rows dr = rr, dy = yr;
+    if (host) {
+      dc = ar.take<uint8_t>(nx);
+      dsc = ar.take<float>(nx / 128u);
+      if (rr.data) dr = device_rows(ar, rr, width, N);
+      dy = device_rows(ar, yr, width, N);
+    }
+    if (pass == 0) continue;
+    if (host) {
+      if ((s = call.stage_in(const_cast<uint8_t *>(dc), codes, nx)) != PW_OK) return s;
+      if ((s = call.stage_in(const_cast<float *>(dsc), scales, nx / 128u * 4u)) != PW_OK) return s;
+      if (rr.data) CK(copy_rows(dr, rr, width, N, cudaMemcpyHostToDevice, rt->stream));
+    }
+    for (uint32_t t0 = 0; t0 < width; t0 += kPiece) {
+      const uint32_t n = width - t0 < kPiece ? width - t0 : kPiece;
+      Descs D;
+      bool cached = false;
+      if ((s = get_descs(rt, 2u, n, chunk, *w, nullptr, nullptr, box_rows, box_kb, D, cached)) != PW_OK) return s;
+      if (!cached) return fail(rt, PW_ERR_UNSUPPORTED, "descriptor slot too small");
+      GemvArgs a = gemv_args(rt, D.gu, D.n_gu, N, K, layout);
+      a.x_codes = dc + (size_t)t0 * K;
+      a.x_scales = dsc + (size_t)t0 * (K / 128u);
+      a.early_weights = chain ? 1u : 0u;
+      a.ep = e;
+      pw_rows pr = dr, py = dy;
+      if (pr.data) pr.data = static_cast<uint8_t *>(pr.data) + t0 * pr.stride * elem_size(pr.dtype);
+      py.data = static_cast<uint8_t *>(py.data) + t0 * py.stride * elem_size(py.dtype);
+      set_rows(a.ep, pr, py);
+      ProfScope ps(rt, P_PROJ, 1);
+      const uint64_t tiles = (uint64_t)D.n_gu * (N / 128u);
+      int grid = grid_for(rt, tiles);
+      if (wide) {
+        GemmArgs A{};
+        A.g = a;
+        if (!encode_act_maps(A.xmap, a.x_codes, n, K))
+          return fail(rt, PW_ERR_CUDA, "cuTensorMapEncodeTiled failed for the activations");
+        CK(launch_gemm_tc(4, A, grid, rt->stream));
+      } else {
+        if ((s = gemv_launch_setup(rt, a, tiles, 1, grid)) != PW_OK) return s;
+        CK(launch_gemv(4, a, grid, rt->stream));
+      }
+    }
+    if (host) CK(copy_rows(yr, dy, width, N, cudaMemcpyDeviceToHost, rt->stream));
+  }
+  return call.finish((uint64_t)N * K + (uint64_t)w->scale_rows * w->scale_cols * 4u);
 }
 
 }  // extern "C"

@@ -38,6 +38,10 @@ ROUTER_F32 = 0
 ROUTER_BF16 = 1
 NORM_F32 = 0
 NORM_BF16 = 1
+NORM_F16 = 2
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PW_DTYPE_*, and PW_NORM_* of the same order
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # PW_ACT_*
+CUDA_STREAM_LEGACY = 1  # cudaStreamLegacy, the handle of the stream that torch calls 0
 
 ERRORS = {
     -1: "argument", -2: "shape", -3: "nonfinite", -4: "device_flags", -5: "cuda", -6: "nccl",
@@ -76,6 +80,21 @@ class Router(ctypes.Structure):
 class Norm(ctypes.Structure):
     _fields_ = [("weight", ctypes.c_void_p), ("hidden", ctypes.c_uint32), ("weight_dtype", ctypes.c_uint32),
                 ("epsilon", ctypes.c_float)]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_uint64), ("dtype", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
+class Dense(ctypes.Structure):
+    _fields_ = [("weight", ctypes.c_void_p), ("stride", ctypes.c_uint64), ("rows", ctypes.c_uint32),
+                ("cols", ctypes.c_uint32), ("dtype", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
+class Epilogue(ctypes.Structure):
+    _fields_ = [("bias", ctypes.c_void_p), ("bias_dtype", ctypes.c_uint32), ("activation", ctypes.c_uint32),
+                ("residual", Rows)]
 
 
 class Stats(ctypes.Structure):
@@ -148,6 +167,15 @@ class Execution:
     weights: Optional[torch.Tensor] = None
 
 
+@dataclass
+class NormExecution:
+    """What add_rms_norm was asked for (None: not asked for)."""
+    sum: Optional[torch.Tensor]
+    y: Optional[torch.Tensor]
+    codes: Optional[torch.Tensor]
+    scales: Optional[torch.Tensor]
+
+
 def _as_f32(x) -> torch.Tensor:
     if isinstance(x, np.ndarray):
         x = torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32))
@@ -204,7 +232,10 @@ class WideMoeRuntime:
         return self._L.pw_last_error(self._rt).decode()
 
     def set_stream(self, stream: Optional[torch.cuda.Stream]) -> None:
-        self._check(self._L.pw_set_stream(self._rt, ctypes.c_void_p(stream.cuda_stream if stream else 0)))
+        """Run later calls on `stream`; None: on the runtime's own stream.  torch's default stream
+        (handle 0, which the C ABI takes for "the runtime's own") goes by its explicit handle."""
+        handle = (stream.cuda_stream or CUDA_STREAM_LEGACY) if stream is not None else 0
+        self._check(self._L.pw_set_stream(self._rt, ctypes.c_void_p(handle)))
 
     def synchronize(self) -> None:
         self._check(self._L.pw_synchronize(self._rt))
@@ -380,6 +411,140 @@ class WideMoeRuntime:
         self._check(self._L.pw_rms_norm(self._rt, ctypes.byref(n), ctypes.c_void_p(x.data_ptr()), x.shape[0],
                                         ctypes.c_void_p(out.data_ptr()), ctypes.c_void_p(inv.data_ptr()), mem, None))
         return out, inv
+
+    # ------------------------------------- residual, norm, linear layers
+    def _rows(self, t: torch.Tensor, name: str, cuda: bool) -> Rows:
+        """pw_rows of a 2-D tensor whose rows are contiguous, on the runtime's device or the host."""
+        if t.dtype not in DTYPES:
+            raise PrismwingError(-1, f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+        if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise PrismwingError(-1, f"{name} must be 2-D with contiguous rows")
+        if t.get_device() != (self.device if cuda else -1):
+            raise PrismwingError(-1, f"{name} is on {t.device}, not with x on the runtime's device or the host")
+        # one row may have any stride in torch
+        return Rows(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, DTYPES[t.dtype], 0)
+
+    def _vector(self, t: torch.Tensor, name: str, n: int) -> int:
+        if t.dtype not in DTYPES or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() \
+                or t.get_device() != self.device:
+            raise PrismwingError(-1, f"{name} must be a contiguous [{n}] float tensor on the runtime's device")
+        return t.data_ptr()
+
+    @staticmethod
+    def _input(x) -> torch.Tensor:
+        if isinstance(x, np.ndarray):
+            x = torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32))
+        return x
+
+    @staticmethod
+    def _mem(x: torch.Tensor, asynchronous: bool):
+        if asynchronous:
+            if not x.is_cuda:
+                raise PrismwingError(-1, "asynchronous calls need device I/O")
+            return MEM_DEVICE | MEM_ASYNC, None
+        return MEM_DEVICE if x.is_cuda else MEM_HOST, Stats()
+
+    def add_rms_norm(self, x, weight: torch.Tensor, epsilon: float = 1e-5, residual=None, want_y: bool = True,
+                     want_codes: bool = False, out_dtype: Optional[torch.dtype] = None, in_place: bool = False,
+                     asynchronous: bool = False) -> NormExecution:
+        """s = x + residual in x's dtype; y = s / sqrt(mean(s^2) + epsilon) * weight, rounded once to out_dtype
+        (x's, or float32); with want_codes y's e4m3 codes (uint8 [rows, hidden]) and their scales per 128 columns
+        (float32 [rows, ceil(hidden / 128)]), taken from y before its rounding.  x, residual [rows, hidden],
+        float32, bfloat16 or float16; weight a CUDA [hidden] of any of them.  in_place writes s over residual."""
+        x = self._input(x)
+        cuda = x.is_cuda
+        xr = self._rows(x, "x", cuda)
+        T, H = x.shape
+        if weight.dtype not in DTYPES:
+            raise PrismwingError(-1, f"norm weight must be float32, bfloat16 or float16, not {weight.dtype}")
+        norm = Norm(self._vector(weight, "norm weight", H), H, DTYPES[weight.dtype], float(epsilon))
+        mem, st = self._mem(x, asynchronous)
+        rr = sr = yr = total = y = codes = scales = None
+        if residual is not None:
+            residual = self._input(residual)
+            rr = self._rows(residual, "residual", cuda)
+            if residual.shape != x.shape:
+                raise PrismwingError(-2, "residual must have x's shape")
+            total = residual if in_place else torch.empty((T, H), dtype=x.dtype, device=x.device)
+            sr = rr if in_place else Rows(total.data_ptr(), H, xr.dtype, 0)
+        if want_y:
+            y = torch.empty((T, H), dtype=out_dtype or x.dtype, device=x.device)
+            yr = self._rows(y, "y", cuda)
+        if want_codes:
+            codes = torch.empty((T, H), dtype=torch.uint8, device=x.device)
+            scales = torch.empty((T, (H + 127) // 128), dtype=torch.float32, device=x.device)
+        ref = ctypes.byref
+        self._check(self._L.pw_add_rms_norm(
+            self._rt, ref(norm), ref(xr), ref(rr) if rr else None, T, ref(sr) if sr else None, ref(yr) if yr else None,
+            codes.data_ptr() if want_codes else None, scales.data_ptr() if want_codes else None, mem,
+            ref(st) if st else None))
+        return NormExecution(total, y, codes, scales)
+
+    def _epilogue(self, x, width: int, cols: int, bias, activation: str, residual, out_dtype, out):
+        """(pw_epilogue, pw_rows of y, y) of a linear layer over `x`'s device or host memory."""
+        if activation not in ACTIVATIONS:
+            raise PrismwingError(-1, f"unknown activation {activation!r}")
+        ep = Epilogue(None, 0, ACTIVATIONS[activation], Rows())
+        if bias is not None:
+            ep.bias = self._vector(bias, "bias", cols)
+            ep.bias_dtype = DTYPES[bias.dtype]
+        if residual is not None:
+            if tuple(residual.shape) != (width, cols):
+                raise PrismwingError(-2, f"residual must be [{width}, {cols}]")
+            ep.residual = self._rows(residual, "residual", x.is_cuda)
+        if out is None:
+            out = torch.empty((width, cols), dtype=out_dtype, device=x.device)
+        elif tuple(out.shape) != (width, cols):
+            raise PrismwingError(-2, f"out must be [{width}, {cols}]")
+        return ep, self._rows(out, "out", x.is_cuda), out
+
+    def linear(self, x, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+               residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+               asynchronous: bool = False, out: Optional[torch.Tensor] = None) -> Execution:
+        """activation(x W^T + bias) + residual for a CUDA bfloat16 or float16 weight [rows, cols] whose rows start at
+        16-byte boundaries (execute_bf16_linear, kernels/block_fp8_gemv.metal:358): sums in 32 bits, rounded once to
+        out_dtype (x's).  x [width, cols] of the weight's dtype, or float32, which is rounded to it first; bias a
+        CUDA [rows], residual [width, rows], of any float dtype; `out` may be `residual`.  activation: "none",
+        "relu", "gelu", "gelu_tanh" or "silu"."""
+        x = self._input(x)
+        xr = self._rows(x, "x", x.is_cuda)
+        wr = self._rows(weight, "weight", True)
+        width, (rows, cols) = x.shape[0], weight.shape
+        if x.shape[1] != cols:
+            raise PrismwingError(-2, f"x has {x.shape[1]} columns, the weight {cols}")
+        mem, st = self._mem(x, asynchronous)
+        ep, yr, out = self._epilogue(x, width, rows, bias, activation, residual, out_dtype or x.dtype, out)
+        w = Dense(wr.data, wr.stride, rows, cols, wr.dtype, 0)
+        ref = ctypes.byref
+        self._check(self._L.pw_linear(self._rt, ref(w), ref(xr), width, ref(ep), ref(yr), mem, ref(st) if st else None))
+        return Execution(out, st.wall_ms if st else 0.0, st.device_ms if st else 0.0,
+                         weight_bytes=st.weight_bytes if st else 0)
+
+    def fp8_linear_codes(self, codes: torch.Tensor, scales: torch.Tensor, binding: WideProjectionBinding,
+                         layout: int = LAYOUT_PLAIN, bias: Optional[torch.Tensor] = None, activation: str = "none",
+                         residual: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
+                         asynchronous: bool = False, out: Optional[torch.Tensor] = None) -> Execution:
+        """execute_fp8_linear on activations that are already quantized (quantize, add_rms_norm), with linear's
+        epilogue: codes uint8 [width, cols], scales float32 [width, cols / 128], both contiguous."""
+        if codes.dtype != torch.uint8 or scales.dtype != torch.float32 or codes.dim() != 2 or scales.dim() != 2:
+            raise PrismwingError(-1, "codes must be uint8 and scales float32, both 2-D")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise PrismwingError(-1, "codes and scales must be contiguous")
+        where = self.device if codes.is_cuda else -1
+        if codes.get_device() != where or scales.get_device() != where:
+            raise PrismwingError(-1, "codes and scales must both be on the runtime's device or the host")
+        width, cols = codes.shape
+        if cols != binding.columns or tuple(scales.shape) != (width, cols // 128):
+            raise PrismwingError(-2, f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit a "
+                                     f"[{binding.rows}, {binding.columns}] projection")
+        mem, st = self._mem(codes, asynchronous)
+        ep, yr, out = self._epilogue(codes, width, binding.rows, bias, activation, residual, out_dtype, out)
+        t = binding.c()
+        ref = ctypes.byref
+        self._check(self._L.pw_fp8_linear_codes(self._rt, ref(t), layout, codes.data_ptr(), scales.data_ptr(), width,
+                                                ref(ep), ref(yr), mem, ref(st) if st else None))
+        return Execution(out, st.wall_ms if st else 0.0, st.device_ms if st else 0.0,
+                         weight_bytes=st.weight_bytes if st else 0)
 
     # ------------------------------------------------------------ layers
     def execute(self, x, experts: Sequence[WideExpertBinding]) -> Execution:
