@@ -54,9 +54,9 @@ __device__ __forceinline__ bool store_elem(void *p, uint64_t i, uint32_t dtype, 
   return finite(__half2float(r));
 }
 
-// The activations from their formulas.  exp(-v) overflows to infinity for
-// v < -88 and the quotient is then -0, the limit; v (1 + erf) / 2 cancels
-// below v ~ -4, so the negative tail is v erfc(-v / sqrt 2) / 2.
+// The activations from their formulas, to a few ulps of f32 (__fdividef: 2).
+// exp(-v) overflows to infinity for v < -88 and the quotient is then -0, the
+// limit; v (1 + erf) / 2 cancels below v ~ -4, so it is v erfc(-v / sqrt 2) / 2.
 __device__ __forceinline__ float activate(float v, uint32_t act) {
   switch (act) {
     case PW_ACT_RELU: return v < 0.0f ? 0.0f : v;  // a NaN stays a NaN
@@ -64,9 +64,9 @@ __device__ __forceinline__ float activate(float v, uint32_t act) {
     case PW_ACT_GELU_TANH: {
       // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
       const float u = 1.5957691216057308f * fmaf(0.044715f * v * v, v, v);
-      return __fdiv_rn(v, 1.0f + expf(-u));
+      return __fdividef(v, 1.0f + expf(-u));
     }
-    case PW_ACT_SILU: return __fdiv_rn(v, 1.0f + expf(-v));
+    case PW_ACT_SILU: return __fdividef(v, 1.0f + expf(-v));
     default: return v;
   }
 }
@@ -79,11 +79,42 @@ __device__ __forceinline__ float epilogue_value(const EpilogueArgs &e, float sum
   return sum;
 }
 
-// Four consecutive columns c .. c + 3 (c % 4 == 0) of token t after bias and
-// activation: adds the residual, rounds and stores, with one access per array
-// where its rows allow.  False when a stored value is not finite.
-__device__ __forceinline__ bool finish4(const EpilogueArgs &e, float4 q, uint64_t t, uint32_t c) {
-  float v[4] = {q.x, q.y, q.z, q.w};
+__device__ __forceinline__ float4 bias4(const EpilogueArgs &e, uint32_t c) {
+  if (!e.bias) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  return make_float4(load_elem(e.bias, c, e.bias_dtype), load_elem(e.bias, c + 1u, e.bias_dtype),
+                     load_elem(e.bias, c + 2u, e.bias_dtype), load_elem(e.bias, c + 3u, e.bias_dtype));
+}
+
+// v[i] = activation(v[i]): one branch for all of them.
+template <int N>
+__device__ __forceinline__ void activate_all(float (&v)[N], uint32_t act) {
+  switch (act) {
+    case PW_ACT_RELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate(v[i], PW_ACT_RELU);
+      break;
+    case PW_ACT_GELU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate(v[i], PW_ACT_GELU);
+      break;
+    case PW_ACT_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate(v[i], PW_ACT_GELU_TANH);
+      break;
+    case PW_ACT_SILU:
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = activate(v[i], PW_ACT_SILU);
+      break;
+    default: break;
+  }
+}
+
+// The epilogue of four consecutive columns c .. c + 3 (c % 4 == 0) of token t,
+// with one access per array where its rows allow.  False when a stored value
+// is not finite.
+__device__ __forceinline__ bool finish4(const EpilogueArgs &e, float4 q, float4 bias, uint64_t t, uint32_t c) {
+  float v[4] = {q.x + bias.x, q.y + bias.y, q.z + bias.z, q.w + bias.w};
+  activate_all(v, e.act);
   const uint32_t rz = e.residual_dtype == PW_DTYPE_F32 ? 4u : 2u, yz = e.y_dtype == PW_DTYPE_F32 ? 4u : 2u;
   if (e.residual) {
     const uint8_t *p = static_cast<const uint8_t *>(e.residual) + (t * e.residual_stride + c) * rz;

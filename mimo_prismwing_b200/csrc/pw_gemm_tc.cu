@@ -423,25 +423,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm_tc(const __grid_constant__
         __syncwarp();  // the staging rows are rewritten by the next piece
       };
       if (KIND == 4) {
-        // The linear layers' epilogue: bias and activation here, where a
-        // thread holds one token's columns; the f32 values then pass through
-        // the staging rows, and the thread that stores four columns of a row
-        // adds the residual and rounds.
+        // The linear layers' epilogue.  The f32 sums pass through the staging
+        // rows 16 columns at a time; the thread that stores four columns of a
+        // row applies bias, activation and residual.  The loop over the rows
+        // stays rolled: unrolled over all 64 values the activations' code
+        // (five formulas each) ran out of the instruction cache and the
+        // epilogue took three times as long as the tile's products.
         const EpilogueArgs &ep = a.ep;
-        if (ep.bias) {
-#pragma unroll
-          for (uint32_t i = 0; i < 32; ++i) {
-            acc[i].x += load_elem(ep.bias, row0 + col0 + 2u * i, ep.bias_dtype);
-            acc[i].y += load_elem(ep.bias, row0 + col0 + 2u * i + 1u, ep.bias_dtype);
-          }
-        }
-        if (ep.act != PW_ACT_NONE) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            acc[i].x = activate(acc[i].x, ep.act);
-            acc[i].y = activate(acc[i].y, ep.act);
-          }
-        }
         bool ok = true;
 #pragma unroll
         for (uint32_t h = 0; h < 4; ++h) {
@@ -451,11 +439,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm_tc(const __grid_constant__
                 make_float4(acc[8 * h + 2 * i].x, acc[8 * h + 2 * i].y, acc[8 * h + 2 * i + 1].x,
                             acc[8 * h + 2 * i + 1].y);
           __syncwarp();
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t r = 8u * j + lane / 4u, c = lane % 4u;
+          const uint32_t c = lane % 4u, col = row0 + col0 + h * 16u + c * 4u;
+          const float4 bias = bias4(ep, col);
+#pragma unroll 1
+          for (uint32_t r = lane / 4u; r < rows_here; r += 8u) {
             const float4 v = *reinterpret_cast<const float4 *>(stg + r * 64u + ((c ^ ((r >> 1) & 3u)) << 4));
-            if (r < rows_here) ok = finish4(ep, v, p0 + r, row0 + col0 + h * 16u + c * 4u) && ok;
+            ok = finish4(ep, v, bias, p0 + r, col) && ok;
           }
           __syncwarp();
         }

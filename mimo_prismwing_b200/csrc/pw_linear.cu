@@ -121,9 +121,7 @@ __device__ __forceinline__ void finish32(const EpilogueArgs &e, float (&v)[32], 
                                          uint32_t n, uint32_t *flags) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] += bias;
-  if (e.act != PW_ACT_NONE)
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = activate(v[j], e.act);
+  activate_all(v, e.act);
   if (e.residual) {
     const uint64_t at = t0 * e.residual_stride + c;
     if (e.residual_dtype == PW_DTYPE_F32) add_rows(v, static_cast<const float *>(e.residual) + at, e.residual_stride, n);

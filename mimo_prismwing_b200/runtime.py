@@ -413,22 +413,35 @@ class WideMoeRuntime:
         return out, inv
 
     # ------------------------------------- residual, norm, linear layers
-    def _rows(self, t: torch.Tensor, name: str, cuda: bool) -> Rows:
-        """pw_rows of a 2-D tensor whose rows are contiguous, on the runtime's device or the host."""
-        if t.dtype not in DTYPES:
+    # These calls take a few microseconds on the device for a single token, so
+    # their host side is kept short: one check per tensor, no conversions.
+    def _rows(self, t: torch.Tensor, name: str, where: int) -> Rows:
+        """pw_rows of a 2-D tensor whose rows are contiguous, on device `where` (-1: the host)."""
+        shape, code = t.shape, DTYPES.get(t.dtype)
+        if len(shape) == 2 and code is not None and t.get_device() == where:
+            rows, cols = shape
+            stride, step = t.stride()
+            if rows <= 1:  # one row may have any stride in torch
+                stride = 0
+            if (step == 1 or cols <= 1) and (stride >= cols or not stride and rows <= 1):
+                return Rows(t.data_ptr(), stride, code, 0)
+        if code is None:
             raise PrismwingError(-1, f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
-        if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-            raise PrismwingError(-1, f"{name} must be 2-D with contiguous rows")
-        if t.get_device() != (self.device if cuda else -1):
+        if t.get_device() != where:
             raise PrismwingError(-1, f"{name} is on {t.device}, not with x on the runtime's device or the host")
-        # one row may have any stride in torch
-        return Rows(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, DTYPES[t.dtype], 0)
+        raise PrismwingError(-1, f"{name} must be 2-D with contiguous rows that do not overlap")
 
     def _vector(self, t: torch.Tensor, name: str, n: int) -> int:
-        if t.dtype not in DTYPES or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() \
-                or t.get_device() != self.device:
+        if t.dtype not in DTYPES or t.shape != (n,) or t.get_device() != self.device or not t.is_contiguous():
             raise PrismwingError(-1, f"{name} must be a contiguous [{n}] float tensor on the runtime's device")
         return t.data_ptr()
+
+    def _where(self, x: torch.Tensor) -> int:
+        """The device index of a call's rows: the runtime's device, or -1 for the host."""
+        where = x.get_device()
+        if where != self.device and where != -1:
+            raise PrismwingError(-1, f"x is on {x.device}, not on the runtime's device or the host")
+        return where
 
     @staticmethod
     def _input(x) -> torch.Tensor:
@@ -437,12 +450,12 @@ class WideMoeRuntime:
         return x
 
     @staticmethod
-    def _mem(x: torch.Tensor, asynchronous: bool):
+    def _mem(where: int, asynchronous: bool):
         if asynchronous:
-            if not x.is_cuda:
+            if where < 0:
                 raise PrismwingError(-1, "asynchronous calls need device I/O")
             return MEM_DEVICE | MEM_ASYNC, None
-        return MEM_DEVICE if x.is_cuda else MEM_HOST, Stats()
+        return MEM_DEVICE if where >= 0 else MEM_HOST, Stats()
 
     def add_rms_norm(self, x, weight: torch.Tensor, epsilon: float = 1e-5, residual=None, want_y: bool = True,
                      want_codes: bool = False, out_dtype: Optional[torch.dtype] = None, in_place: bool = False,
@@ -452,51 +465,67 @@ class WideMoeRuntime:
         (float32 [rows, ceil(hidden / 128)]), taken from y before its rounding.  x, residual [rows, hidden],
         float32, bfloat16 or float16; weight a CUDA [hidden] of any of them.  in_place writes s over residual."""
         x = self._input(x)
-        cuda = x.is_cuda
-        xr = self._rows(x, "x", cuda)
+        where = self._where(x)
+        xr = self._rows(x, "x", where)
         T, H = x.shape
+        dtype, dev = x.dtype, x.device
         if weight.dtype not in DTYPES:
             raise PrismwingError(-1, f"norm weight must be float32, bfloat16 or float16, not {weight.dtype}")
-        norm = Norm(self._vector(weight, "norm weight", H), H, DTYPES[weight.dtype], float(epsilon))
-        mem, st = self._mem(x, asynchronous)
-        rr = sr = yr = total = y = codes = scales = None
+        norm = Norm(self._vector(weight, "norm weight", H), H, DTYPES[weight.dtype], epsilon)
+        mem, st = self._mem(where, asynchronous)
+        ref, empty = ctypes.byref, torch.empty_strided
+        rr = sr = yr = cp = sp = total = y = codes = scales = None
         if residual is not None:
             residual = self._input(residual)
-            rr = self._rows(residual, "residual", cuda)
+            res = self._rows(residual, "residual", where)
             if residual.shape != x.shape:
                 raise PrismwingError(-2, "residual must have x's shape")
-            total = residual if in_place else torch.empty((T, H), dtype=x.dtype, device=x.device)
-            sr = rr if in_place else Rows(total.data_ptr(), H, xr.dtype, 0)
+            rr = ref(res)
+            if in_place:
+                total, sr = residual, rr
+            else:
+                total = empty((T, H), (H, 1), dtype=dtype, device=dev)
+                sr = ref(Rows(total.data_ptr(), H, xr.dtype, 0))
         if want_y:
-            y = torch.empty((T, H), dtype=out_dtype or x.dtype, device=x.device)
-            yr = self._rows(y, "y", cuda)
+            if out_dtype is None:
+                out_dtype = dtype
+            elif out_dtype not in DTYPES:
+                raise PrismwingError(-1, f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+            y = empty((T, H), (H, 1), dtype=out_dtype, device=dev)
+            yr = ref(Rows(y.data_ptr(), H, DTYPES[out_dtype], 0))
         if want_codes:
-            codes = torch.empty((T, H), dtype=torch.uint8, device=x.device)
-            scales = torch.empty((T, (H + 127) // 128), dtype=torch.float32, device=x.device)
-        ref = ctypes.byref
-        self._check(self._L.pw_add_rms_norm(
-            self._rt, ref(norm), ref(xr), ref(rr) if rr else None, T, ref(sr) if sr else None, ref(yr) if yr else None,
-            codes.data_ptr() if want_codes else None, scales.data_ptr() if want_codes else None, mem,
-            ref(st) if st else None))
+            G = (H + 127) // 128
+            codes = empty((T, H), (H, 1), dtype=torch.uint8, device=dev)
+            scales = empty((T, G), (G, 1), dtype=torch.float32, device=dev)
+            cp, sp = codes.data_ptr(), scales.data_ptr()
+        status = self._L.pw_add_rms_norm(self._rt, ref(norm), ref(xr), rr, T, sr, yr, cp, sp, mem,
+                                         ref(st) if st else None)
+        if status:
+            self._check(status)
         return NormExecution(total, y, codes, scales)
 
-    def _epilogue(self, x, width: int, cols: int, bias, activation: str, residual, out_dtype, out):
-        """(pw_epilogue, pw_rows of y, y) of a linear layer over `x`'s device or host memory."""
-        if activation not in ACTIVATIONS:
+    def _epilogue(self, where: int, dev, width: int, cols: int, bias, activation: str, residual, out_dtype, out):
+        """(pw_epilogue, pw_rows of y, y) of a linear layer over rows on device `where`."""
+        act = ACTIVATIONS.get(activation)
+        if act is None:
             raise PrismwingError(-1, f"unknown activation {activation!r}")
-        ep = Epilogue(None, 0, ACTIVATIONS[activation], Rows())
+        ep = Epilogue(None, 0, act)
         if bias is not None:
             ep.bias = self._vector(bias, "bias", cols)
             ep.bias_dtype = DTYPES[bias.dtype]
         if residual is not None:
-            if tuple(residual.shape) != (width, cols):
+            if residual.shape != (width, cols):
                 raise PrismwingError(-2, f"residual must be [{width}, {cols}]")
-            ep.residual = self._rows(residual, "residual", x.is_cuda)
-        if out is None:
-            out = torch.empty((width, cols), dtype=out_dtype, device=x.device)
-        elif tuple(out.shape) != (width, cols):
-            raise PrismwingError(-2, f"out must be [{width}, {cols}]")
-        return ep, self._rows(out, "out", x.is_cuda), out
+            ep.residual = self._rows(residual, "residual", where)
+        if out is not None:
+            if out.shape != (width, cols):
+                raise PrismwingError(-2, f"out must be [{width}, {cols}]")
+            return ep, self._rows(out, "out", where), out
+        code = DTYPES.get(out_dtype)
+        if code is None:
+            raise PrismwingError(-1, f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+        out = torch.empty_strided((width, cols), (cols, 1), dtype=out_dtype, device=dev)
+        return ep, Rows(out.data_ptr(), cols, code, 0), out
 
     def linear(self, x, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
                residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
@@ -507,18 +536,23 @@ class WideMoeRuntime:
         CUDA [rows], residual [width, rows], of any float dtype; `out` may be `residual`.  activation: "none",
         "relu", "gelu", "gelu_tanh" or "silu"."""
         x = self._input(x)
-        xr = self._rows(x, "x", x.is_cuda)
-        wr = self._rows(weight, "weight", True)
-        width, (rows, cols) = x.shape[0], weight.shape
-        if x.shape[1] != cols:
-            raise PrismwingError(-2, f"x has {x.shape[1]} columns, the weight {cols}")
-        mem, st = self._mem(x, asynchronous)
-        ep, yr, out = self._epilogue(x, width, rows, bias, activation, residual, out_dtype or x.dtype, out)
+        where = self._where(x)
+        xr = self._rows(x, "x", where)
+        wr = self._rows(weight, "weight", self.device)
+        rows, cols = weight.shape
+        width, columns = x.shape
+        if columns != cols:
+            raise PrismwingError(-2, f"x has {columns} columns, the weight {cols}")
+        mem, st = self._mem(where, asynchronous)
+        ep, yr, out = self._epilogue(where, x.device, width, rows, bias, activation, residual, out_dtype or x.dtype, out)
         w = Dense(wr.data, wr.stride, rows, cols, wr.dtype, 0)
         ref = ctypes.byref
-        self._check(self._L.pw_linear(self._rt, ref(w), ref(xr), width, ref(ep), ref(yr), mem, ref(st) if st else None))
-        return Execution(out, st.wall_ms if st else 0.0, st.device_ms if st else 0.0,
-                         weight_bytes=st.weight_bytes if st else 0)
+        status = self._L.pw_linear(self._rt, ref(w), ref(xr), width, ref(ep), ref(yr), mem, ref(st) if st else None)
+        if status:
+            self._check(status)
+        if st is None:
+            return Execution(out, 0.0, 0.0)
+        return Execution(out, st.wall_ms, st.device_ms, weight_bytes=st.weight_bytes)
 
     def fp8_linear_codes(self, codes: torch.Tensor, scales: torch.Tensor, binding: WideProjectionBinding,
                          layout: int = LAYOUT_PLAIN, bias: Optional[torch.Tensor] = None, activation: str = "none",
@@ -530,21 +564,26 @@ class WideMoeRuntime:
             raise PrismwingError(-1, "codes must be uint8 and scales float32, both 2-D")
         if not (codes.is_contiguous() and scales.is_contiguous()):
             raise PrismwingError(-1, "codes and scales must be contiguous")
-        where = self.device if codes.is_cuda else -1
-        if codes.get_device() != where or scales.get_device() != where:
+        where = self._where(codes)
+        if scales.get_device() != where:
             raise PrismwingError(-1, "codes and scales must both be on the runtime's device or the host")
         width, cols = codes.shape
-        if cols != binding.columns or tuple(scales.shape) != (width, cols // 128):
-            raise PrismwingError(-2, f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit a "
-                                     f"[{binding.rows}, {binding.columns}] projection")
-        mem, st = self._mem(codes, asynchronous)
-        ep, yr, out = self._epilogue(codes, width, binding.rows, bias, activation, residual, out_dtype, out)
         t = binding.c()
+        if binding.weight.get_device() != self.device or binding.scale.get_device() != self.device:
+            raise PrismwingError(-1, "the projection is not on the runtime's device")
+        if cols != t.cols or scales.shape != (width, cols // 128):
+            raise PrismwingError(-2, f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit a "
+                                     f"[{t.rows}, {t.cols}] projection")
+        mem, st = self._mem(where, asynchronous)
+        ep, yr, out = self._epilogue(where, codes.device, width, t.rows, bias, activation, residual, out_dtype, out)
         ref = ctypes.byref
-        self._check(self._L.pw_fp8_linear_codes(self._rt, ref(t), layout, codes.data_ptr(), scales.data_ptr(), width,
-                                                ref(ep), ref(yr), mem, ref(st) if st else None))
-        return Execution(out, st.wall_ms if st else 0.0, st.device_ms if st else 0.0,
-                         weight_bytes=st.weight_bytes if st else 0)
+        status = self._L.pw_fp8_linear_codes(self._rt, ref(t), layout, codes.data_ptr(), scales.data_ptr(), width,
+                                             ref(ep), ref(yr), mem, ref(st) if st else None)
+        if status:
+            self._check(status)
+        if st is None:
+            return Execution(out, 0.0, 0.0)
+        return Execution(out, st.wall_ms, st.device_ms, weight_bytes=st.weight_bytes)
 
     # ------------------------------------------------------------ layers
     def execute(self, x, experts: Sequence[WideExpertBinding]) -> Execution:
