@@ -13,8 +13,6 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
-
 #include "pw_device.cuh"
 #include "pw_epilogue.cuh"
 #include "pw_internal.h"
@@ -305,20 +303,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
   tc_fence_after();
   if (warp == (uint32_t)kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
-}
-
-// Raises a kernel's shared-memory limit once per device.
-template <auto Kernel>
-cudaError_t allow_smem(uint32_t bytes) {
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
-  return e;
 }
 
 template <int BN>

@@ -996,6 +996,7 @@ int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const
   const uint32_t H = norm->hidden;
   if (H == 0 || H > 16384u) return fail(rt, PW_ERR_SHAPE, "RMSNorm shape mismatch (hidden %u, 1 to 16384)", H);
   if (rows == 0) return fail(rt, PW_ERR_SHAPE, "RMSNorm needs at least one row");
+  if (rows > (1u << 30)) return fail(rt, PW_ERR_UNSUPPORTED, "too many rows");
   if (!codes != !scales) return fail(rt, PW_ERR_ARGUMENT, "codes and scales go together");
   if (!y && !codes) return fail(rt, PW_ERR_ARGUMENT, "nothing asked for: neither y nor codes");
   if (reinterpret_cast<uintptr_t>(scales) % 4u) return fail(rt, PW_ERR_ARGUMENT, "scales are not aligned to their elements");

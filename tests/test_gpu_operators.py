@@ -102,6 +102,23 @@ def test_norm_matches_its_definition(rt, rows, hidden, dtype):
     close(rt.add_rms_norm(x, w, 1e-5, residual=r, out_dtype=torch.float32).y, y, torch.float32, NORM_TOL)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,hidden,residual", [(4001, 512, True), (2500, 4096, True), (2500, 4096, False),
+                                                  (700, 8192, True), (400, 16384, False), (300, 16384, True)])
+def test_norm_over_many_rows(rt, rows, hidden, residual, dtype):
+    # several rows per CTA, in place over the stream
+    t = TYPES[dtype]
+    x, _ = wide(randn((rows, hidden), 13, t, 3.0), 8)
+    r = randn((rows, hidden), 14, t, 3.0) if residual else None
+    w = randn((hidden,), 15) + 1
+    s, y = norm_reference(x, r, w, 1e-5)
+    got = rt.add_rms_norm(x, w, 1e-5, residual=r, want_codes=True, in_place=residual)
+    if residual:
+        assert torch.equal(r, s)
+    close(got.y, y, t, NORM_TOL)
+    check_codes(got.codes, got.scales, y)
+
+
 @pytest.mark.parametrize("wtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("pad", [1, 3, 8])
 def test_norm_strides_and_weight_types(rt, pad, wtype):
