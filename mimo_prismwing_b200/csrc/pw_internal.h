@@ -271,6 +271,8 @@ struct LinearArgs {
   uint32_t *flags;
 };
 cudaError_t launch_linear(const LinearArgs &a, int num_sms, cudaStream_t stream);
+// up to 16 tokens (pw_linear_narrow.cu)
+cudaError_t launch_linear_narrow(const LinearArgs &a, int num_sms, cudaStream_t stream);
 // out[r, c] (rows of `out_stride` elements of 16-bit dtype) = x[r, c]
 // converted from x_dtype.
 cudaError_t launch_convert_rows(const void *x, uint64_t x_stride, uint32_t x_dtype, uint32_t rows, uint32_t cols,

@@ -10,6 +10,7 @@
 // issues tcgen05.mma.kind::f16 into one of two TMEM accumulators, eight
 // epilogue warps empty the other.  Sums are f32 over the whole K.
 #include <cstdint>
+#include <cstdlib>
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -354,6 +355,7 @@ cudaError_t launch_convert_rows(const void *x, uint64_t x_stride, uint32_t x_dty
 cudaError_t launch_linear(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   if (a.rows == 0 || a.cols == 0 || (a.dtype != PW_DTYPE_BF16 && a.dtype != PW_DTYPE_F16)) return cudaErrorInvalidValue;
   if (a.width == 0) return cudaSuccess;
+  if (a.width <= 16u && !getenv("PW_NONARROW")) return launch_linear_narrow(a, num_sms, stream);
   if (a.width <= 32u) return lin::launch_tc<32>(a, num_sms, stream);
   if (a.width <= 64u) return lin::launch_tc<64>(a, num_sms, stream);
   if (a.width <= 128u) return lin::launch_tc<128>(a, num_sms, stream);

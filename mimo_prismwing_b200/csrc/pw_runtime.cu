@@ -1075,6 +1075,7 @@ int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const
     a.flags = rt->d_flags;
     {
       ProfScope ps(rt, P_QUANT, 1);
+      PdlScope pdl(!rt->profiling);
       CK(launch_add_norm(a, rt->num_sms, rt->stream));
     }
     if (call.host()) {
@@ -1160,6 +1161,7 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
     a.flags = rt->d_flags;
     {
       ProfScope ps(rt, P_PROJ, 1);
+      PdlScope pdl(!rt->profiling);
       CK(launch_linear(a, rt->num_sms, rt->stream));
     }
     if (call.host()) CK(copy_rows(yr, dy, width, N, cudaMemcpyDeviceToHost, rt->stream));
