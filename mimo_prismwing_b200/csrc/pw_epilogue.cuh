@@ -54,13 +54,36 @@ __device__ __forceinline__ bool store_elem(void *p, uint64_t i, uint32_t dtype, 
   return finite(__half2float(r));
 }
 
-// The activations from their formulas, to a few ulps of f32 (__fdividef: 2).
-// exp(-v) overflows to infinity for v < -88 and the quotient is then -0, the
-// limit; v (1 + erf) / 2 cancels below v ~ -4, so it is v erfc(-v / sqrt 2) / 2.
+// The activations from their formulas, to a few ulps of f32 (__fdividef: 2),
+// without branches, so that the compiler interleaves several values.
+// exp(-v) overflows to infinity for v < -88 and the quotient is then -0, the limit.
+//
+// GELU: v (1 + erf(v / sqrt 2)) / 2 cancels below v ~ -4, so with z = |v| / sqrt 2
+// it is h = v erfc(z) / 2 for v < 0 and v - h for v > 0.  erfc(z) = exp(-z^2) t Q(t),
+// t = 1 / (1 + 0.4 z): Q is a degree-8 polynomial fitted here to exp(z^2) erfc(z) / t
+// over z in [0, 10.5] by iteratively reweighted least squares in relative error
+// (largest 6.6e-8; with f32 arithmetic 5.5e-7 for |v| < 3, growing with v^2 2^-24
+// in the tail).  CUDA's erfcf has branches that kept the values of a thread from
+// overlapping: a 8192 x 16384 x 4096 layer took 877 us with it, 709 us without
+// an activation.
+__device__ __forceinline__ float gelu(float v) {
+  const float t = __fdividef(1.0f, fmaf(0.4f * 0.70710678f, fabsf(v), 1.0f));
+  float q = 0.04211849719f;
+  q = fmaf(q, t, -0.1445513666f);
+  q = fmaf(q, t, 0.09278277308f);
+  q = fmaf(q, t, 0.07784505188f);
+  q = fmaf(q, t, 0.08678550273f);
+  q = fmaf(q, t, 0.190383628f);
+  q = fmaf(q, t, 0.202661037f);
+  q = fmaf(q, t, 0.2263343185f);
+  q = fmaf(q, t, 0.2256406248f);
+  const float h = 0.5f * v * (exp2f(-0.72134752f * v * v) * (t * q));
+  return v < 0.0f ? h : v - h;
+}
 __device__ __forceinline__ float activate(float v, uint32_t act) {
   switch (act) {
     case PW_ACT_RELU: return v < 0.0f ? 0.0f : v;  // a NaN stays a NaN
-    case PW_ACT_GELU: return 0.5f * v * erfcf(-0.70710678118654752f * v);
+    case PW_ACT_GELU: return gelu(v);
     case PW_ACT_GELU_TANH: {
       // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
       const float u = 1.5957691216057308f * fmaf(0.044715f * v * v, v, v);

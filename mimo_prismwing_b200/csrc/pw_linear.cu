@@ -1,16 +1,29 @@
 // pw_linear.cu -- linear layer over a 16-bit weight on tcgen05 / TMEM:
 //   y[t, r] = round(act(sum_c x[t, c] W[r, c] + bias[r]) + residual[t, r]).
 //
-// A tile is 128 weight rows (TMEM lanes) x BN tokens (TMEM columns): A = W,
-// B = x, both K-major in shared memory (128B swizzle, written by TMA, zero
-// past the matrices' ends, so no size is special).  With weight rows on the
-// lanes a warp's store covers 32 consecutive outputs of one token, whatever
-// the output's stride or alignment, and the bias is one value per thread.
-// Persistent CTAs, one per SM: a producer warp fills the TMA ring, an MMA warp
-// issues tcgen05.mma.kind::f16 into one of two TMEM accumulators, eight
-// epilogue warps empty the other.  Sums are f32 over the whole K.
+// Weight rows are the TMEM lanes (A), tokens the columns (B), both K-major in
+// shared memory (128B swizzle, written by TMA, zero past the matrices' ends, so
+// no size is special).  With weight rows on the lanes a warp's store covers 32
+// consecutive outputs of one token, whatever the output's stride or alignment,
+// and the bias is one value per thread.  In both kernels a producer warp fills
+// the TMA ring, an MMA warp issues tcgen05.mma.kind::f16 into TMEM accumulators,
+// and eight epilogue warps empty them.
+//
+//  * k_linear_pair, for many tokens and 16-bit outputs: two CTAs on one 256 x 256
+//    tile (cta_group::2): each holds its 128 weight rows and half of the tokens,
+//    so the shared memory that a tensor core reads per product is half of what a
+//    128 x 256 tile of one CTA needs.  Persistent pairs, two accumulators, the
+//    whole K in one accumulator.  Bound by the tensor pipe.
+//  * k_linear_tile, for the widths between and for f32 outputs: 128 x 32, 64 or
+//    128 tiles of one CTA.  K runs in segments of 512 columns: each gets a fresh
+//    accumulator, and the epilogue adds the segments in registers.  (The tensor
+//    pipe truncates when it adds to an accumulator: over 4096 columns in one
+//    accumulator an f32 result was 4.4e-6 off, with segments it is below 1e-6; a
+//    16-bit result does not show it.)  When the tiles are fewer than the SMs, the
+//    CTAs of a cluster split K and exchange their sums through distributed shared
+//    memory, each finishing its share of the tokens: HBM bounds these widths, and
+//    a stream over a third of the SMs does not reach it.
 #include <cstdint>
-#include <cstdlib>
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -36,26 +49,44 @@ constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kBlockK = 64;        // columns of a k-block: one 128-byte line
 constexpr uint32_t kSmemLimit = 227u * 1024u;
 constexpr uint32_t kTokenGroup = 8;     // token tiles that neighbouring CTAs share weights over
+constexpr uint32_t kMaxSplits = 8;
 
 template <int BN>
-struct Cfg {
-  static constexpr uint32_t KBS = BN == 256 ? 1u : 2u;  // k-blocks per stage
+struct TileCfg {
+  static constexpr uint32_t KBS = 2;  // k-blocks per stage: 32 KB of weights per TMA box
   static constexpr uint32_t A_BYTES = KBS * kTileRows * 128u;
   static constexpr uint32_t B_BYTES = KBS * (uint32_t)BN * 128u;
   static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
   static constexpr uint32_t NST = (kSmemLimit - 2048u) / STAGE < 6u ? (kSmemLimit - 2048u) / STAGE : 6u;
+  static constexpr uint32_t NACC = 4;    // accumulators: segments in flight
+  static constexpr uint32_t SEG = 4;     // stages per segment: 512 columns
+  static constexpr uint32_t BARS = NST * STAGE;
+  static constexpr uint32_t MISC = BARS + (2u * NST + 2u * NACC) * 8u;
+  static constexpr uint32_t SMEM = MISC + 16u + 1024u;  // + alignment slack
+  static constexpr uint32_t TMEM_COLS = NACC * (uint32_t)BN;
+  static_assert(SMEM <= kSmemLimit, "shared memory");
+  // the K splits' exchange reuses the ring: [split][token of the share][128 rows] f32
+  static_assert(((uint32_t)BN + kMaxSplits) * kTileRows * 4u <= NST * STAGE, "exchange buffer");
+};
+
+struct PairCfg {
+  static constexpr uint32_t BN = 256;               // tokens of the pair's tile, half of them per CTA
+  static constexpr uint32_t A_BYTES = kTileRows * 128u;
+  static constexpr uint32_t B_BYTES = BN / 2u * 128u;
+  static constexpr uint32_t STAGE = A_BYTES + B_BYTES;  // one k-block
+  static constexpr uint32_t NST = 7;
   static constexpr uint32_t BARS = NST * STAGE;
   static constexpr uint32_t MISC = BARS + (2u * NST + 4u) * 8u;
-  static constexpr uint32_t SMEM = MISC + 16u + 1024u;  // + alignment slack
-  static constexpr uint32_t TMEM_COLS = 2u * (uint32_t)BN;
+  static constexpr uint32_t SMEM = MISC + 16u + 1024u;
+  static constexpr uint32_t TMEM_COLS = 2u * BN;
   static_assert(SMEM <= kSmemLimit, "shared memory");
 };
 
 struct Args {
   LinearArgs a;
   CUtensorMap wmap, xmap;
-  uint32_t w3d, x3d;  // the maps have a k-block dimension (encode_rows16_map)
-  uint32_t row_tiles, token_tiles, stages;
+  uint32_t k3d;  // the maps have a k-block dimension (encode_rows16_map)
+  uint32_t row_tiles, token_tiles, stages, splits;
 };
 
 // kind::f16 instruction descriptor: D f32, A and B both bf16 or both f16, K-major.
@@ -75,6 +106,57 @@ __device__ __forceinline__ void mma_f16_elect(uint32_t d, uint64_t a, uint64_t b
       : "memory");
 }
 
+// The pair's MMA (M = 256 over both CTAs, N = 256), issued in the leading CTA.
+__device__ __forceinline__ void mma_f16_pair_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accum)
+      : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs once the MMAs so far are complete.
+__device__ __forceinline__ void mma_commit_pair_elect(uint64_t *bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
+          smem_addr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+// A tile load into this CTA's shared memory that completes on the pair's
+// leading CTA's barrier (a shared::cluster address).
+__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+      "%4}], [%5];" ::"r"(smem_addr(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The address of this CTA's shared-memory location in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void store_remote(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 struct Shared {
   uint8_t *ring;
   uint64_t *full, *empty, *tfull, *tempty;
@@ -82,9 +164,40 @@ struct Shared {
   volatile int *abort;
 };
 
+// Bounded wait (1 s) that sleeps in hardware between looks: ten warps polling in
+// a loop took a fifth of the ALU's issue slots and, under the power cap, clock
+// from the tensor pipe.  PAIR: the pair's other CTA arrives on the barrier too.
+template <bool PAIR>
+__device__ __forceinline__ bool try_wait_sleep(uint64_t *bar, uint32_t parity) {
+  constexpr uint32_t kSleepNs = 100000;  // at most; the phase's completion wakes the thread
+  uint32_t done;
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(kSleepNs)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(kSleepNs)
+        : "memory");
+  return done != 0u;
+}
+
+template <bool PAIR = false>
 __device__ __forceinline__ bool lwait(const Shared &sh, uint64_t *bar, uint32_t parity, uint32_t *flags) {
   if (*sh.abort) return false;
-  if (mbar_wait(bar, parity)) return true;
+  if (try_wait_sleep<PAIR>(bar, parity)) return true;
+  const uint64_t start = global_timer_ns();
+  do {
+    if (try_wait_sleep<PAIR>(bar, parity)) return true;
+  } while (global_timer_ns() - start <= kWaitLimitNs);
   *sh.abort = 1;
   raise_flag(flags, PW_FLAG_WAIT_TIMEOUT);
   return false;
@@ -99,13 +212,34 @@ __device__ __forceinline__ void tile_of(const Args &A, uint32_t u, uint32_t &row
   token_tile = g * kTokenGroup + in % width;
 }
 
-template <typename T>
-__device__ __forceinline__ void add_rows(float (&v)[32], const T *p, uint64_t stride, uint32_t n) {
-  float r[32];
+// The residual of output column c, tokens t0 .. t0 + n - 1 (n >= 1): loads only,
+// all 32 in flight, so they can be issued before what they are added to is ready.
+// Past the last token they repeat it.
+__device__ __forceinline__ void load_residual32(const EpilogueArgs &e, uint64_t t0, uint32_t c, uint32_t n,
+                                                uint32_t (&raw)[32]) {
+  const uint64_t at = t0 * e.residual_stride + c;
+  if (e.residual_dtype == PW_DTYPE_F32) {
+    const uint32_t *p = static_cast<const uint32_t *>(e.residual) + at;
 #pragma unroll
-  for (uint32_t j = 0; j < 32; ++j) r[j] = j < n ? to_f32(p[j * stride]) : 0.0f;
+    for (uint32_t j = 0; j < 32; ++j) raw[j] = p[min(j, n - 1u) * e.residual_stride];
+  } else {
+    const uint16_t *p = static_cast<const uint16_t *>(e.residual) + at;
 #pragma unroll
-  for (uint32_t j = 0; j < 32; ++j) v[j] += r[j];
+    for (uint32_t j = 0; j < 32; ++j) raw[j] = p[min(j, n - 1u) * e.residual_stride];
+  }
+}
+
+__device__ __forceinline__ void add_residual32(const EpilogueArgs &e, const uint32_t (&raw)[32], float (&v)[32]) {
+  if (e.residual_dtype == PW_DTYPE_F32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(raw[j]);
+  } else if (e.residual_dtype == PW_DTYPE_BF16) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(raw[j] << 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += __half2float(__ushort_as_half((unsigned short)raw[j]));
+  }
 }
 
 template <typename T>
@@ -115,19 +249,14 @@ __device__ __forceinline__ void store_rows(const float (&v)[32], T *p, uint64_t 
     if (j < n) p[j * stride] = from_f32<T>(v[j]);
 }
 
-// The epilogue of one thread: output column c of tokens t0 .. t0 + n - 1.
-__device__ __forceinline__ void finish32(const EpilogueArgs &e, float (&v)[32], float bias, uint64_t t0, uint32_t c,
-                                         uint32_t n, uint32_t *flags) {
+// The epilogue of one thread: output column c of tokens t0 .. t0 + n - 1, raw its
+// residual (load_residual32).
+__device__ __forceinline__ void finish32(const EpilogueArgs &e, float (&v)[32], float bias, const uint32_t (&raw)[32],
+                                         uint64_t t0, uint32_t c, uint32_t n, uint32_t *flags) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] += bias;
   activate_all(v, e.act);
-  if (e.residual) {
-    const uint64_t at = t0 * e.residual_stride + c;
-    if (e.residual_dtype == PW_DTYPE_F32) add_rows(v, static_cast<const float *>(e.residual) + at, e.residual_stride, n);
-    else if (e.residual_dtype == PW_DTYPE_BF16)
-      add_rows(v, static_cast<const __nv_bfloat16 *>(e.residual) + at, e.residual_stride, n);
-    else add_rows(v, static_cast<const __half *>(e.residual) + at, e.residual_stride, n);
-  }
+  if (e.residual) add_residual32(e, raw, v);
   uint32_t top = 0u;
 #pragma unroll
   for (uint32_t j = 0; j < 32; ++j)
@@ -140,9 +269,9 @@ __device__ __forceinline__ void finish32(const EpilogueArgs &e, float (&v)[32], 
 }
 
 template <int BN>
-__global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant__ Args A) {
-  using C = Cfg<BN>;
-  constexpr uint32_t NST = C::NST;
+__global__ void __launch_bounds__(kThreads, 1) k_linear_tile(const __grid_constant__ Args A) {
+  using C = TileCfg<BN>;
+  constexpr uint32_t NST = C::NST, NACC = C::NACC;
   const LinearArgs &a = A.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -151,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
   sh.full = reinterpret_cast<uint64_t *>(smem + C::BARS);
   sh.empty = sh.full + NST;
   sh.tfull = sh.empty + NST;
-  sh.tempty = sh.tfull + 2;
+  sh.tempty = sh.tfull + NACC;
   sh.tmem_base = reinterpret_cast<uint32_t *>(smem + C::MISC);
   sh.abort = reinterpret_cast<volatile int *>(smem + C::MISC + 4);
 
@@ -161,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
       mbar_init(&sh.full[i], 1);
       mbar_init(&sh.empty[i], 1);  // tcgen05.commit after the stage's MMAs
     }
-    for (uint32_t i = 0; i < 2; ++i) {
-      mbar_init(&sh.tfull[i], 1);           // tcgen05.commit after the tile's MMAs
+    for (uint32_t i = 0; i < NACC; ++i) {
+      mbar_init(&sh.tfull[i], 1);           // tcgen05.commit after the segment's MMAs
       mbar_init(&sh.tempty[i], kEpiWarps);  // one arrive per epilogue warp
     }
     *sh.abort = 0;
@@ -180,34 +309,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
   pdl_wait();
   pdl_launch_dependents();
   const uint32_t tmem = *sh.tmem_base;
+  // A cluster takes a tile, its CTA `rank` the K stages [st0, st1).  With K
+  // splits there is one tile per cluster (the exchange reuses the ring).
   const uint32_t total = A.row_tiles * A.token_tiles;
+  const uint32_t splits = A.splits, rank = blockIdx.x % splits;
+  const uint32_t u_begin = blockIdx.x / splits, u_step = gridDim.x / splits;
+  const uint32_t st0 = A.stages * rank / splits, st1 = A.stages * (rank + 1u) / splits;
 
   if (warp == (uint32_t)kProducerWarp) {
     uint32_t slot = 0, phase = 0, issued = 0, parity = 0;
-    for (uint32_t u = blockIdx.x; u < total; u += gridDim.x) {
+    for (uint32_t u = u_begin; u < total; u += u_step) {
       uint32_t rt, tt;
       tile_of(A, u, rt, tt);
       const int row0 = (int)(rt * kTileRows), tok0 = (int)(tt * BN);
-      for (uint32_t st = 0; st < A.stages; ++st) {
+      for (uint32_t st = st0; st < st1; ++st) {
         if (lwait(sh, &sh.empty[slot], phase ^ 1u, a.flags)) {
           uint8_t *dst = sh.ring + slot * C::STAGE;
           const int kb = (int)(st * C::KBS);
           if (elect_one()) {
             mbar_arrive_expect_tx(&sh.full[slot], C::STAGE);
-            if (A.w3d) {
+            if (A.k3d) {
               tc::tma_load_3d(dst, &A.wmap, 0, row0, kb, &sh.full[slot]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < (int)C::KBS; ++j)
-                tc::tma_load_3d(dst + j * (kTileRows * 128u), &A.wmap, (kb + j) * (int)kBlockK, row0, 0, &sh.full[slot]);
-            }
-            if (A.x3d) {
               tc::tma_load_3d(dst + C::A_BYTES, &A.xmap, 0, tok0, kb, &sh.full[slot]);
             } else {
 #pragma unroll
-              for (int j = 0; j < (int)C::KBS; ++j)
+              for (int j = 0; j < (int)C::KBS; ++j) {
+                tc::tma_load_3d(dst + j * (kTileRows * 128u), &A.wmap, (kb + j) * (int)kBlockK, row0, 0, &sh.full[slot]);
                 tc::tma_load_3d(dst + C::A_BYTES + j * (BN * 128u), &A.xmap, (kb + j) * (int)kBlockK, tok0, 0,
                                 &sh.full[slot]);
+              }
             }
           }
           __syncwarp();
@@ -228,14 +358,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     const uint32_t idesc = instr_desc16(BN, kTileRows, a.dtype == PW_DTYPE_BF16);
     const uint64_t ring_desc = smem_desc_sw128(smem_addr(sh.ring));
     uint32_t slot = 0, phase = 0, acc = 0, aphase = 0, pending = 0, pend_parity = 0;
-    for (uint32_t u = blockIdx.x; u < total; u += gridDim.x) {
-      const bool ok_acc = lwait(sh, &sh.tempty[acc], aphase ^ 1u, a.flags);
-      tc_fence_after();
-      const uint32_t d = tmem + acc * (uint32_t)BN;
-      for (uint32_t st = 0; st < A.stages; ++st) {
+    for (uint32_t u = u_begin; u < total; u += u_step) {
+      bool ok_acc = true;
+      for (uint32_t st = st0; st < st1; ++st) {
+        const uint32_t in_seg = (st - st0) % C::SEG;
+        if (in_seg == 0u) {
+          ok_acc = lwait(sh, &sh.tempty[acc], aphase ^ 1u, a.flags);
+          tc_fence_after();
+        }
         const bool ok = lwait(sh, &sh.full[slot], phase, a.flags) && ok_acc;
         tc_fence_after();
         if (ok) {
+          const uint32_t d = tmem + acc * (uint32_t)BN;
           const uint64_t ad = ring_desc + ((slot * C::STAGE) >> 4);
           const uint64_t bd = ad + (C::A_BYTES >> 4);
 #pragma unroll
@@ -243,60 +377,125 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
 #pragma unroll
             for (uint32_t s = 0; s < 4; ++s)
               mma_f16_elect(d, ad + ((j * kTileRows * 128u) >> 4) + 2u * s, bd + ((j * BN * 128u) >> 4) + 2u * s, idesc,
-                            (st | j | s) ? 1u : 0u);
+                            (in_seg | j | s) ? 1u : 0u);
         }
         tc::mma_commit_elect(&sh.empty[slot]);
         if (++slot == NST) {
           slot = 0;
           phase ^= 1u;
         }
-      }
-      tc::mma_commit_elect(&sh.tfull[acc]);
-      pending |= 1u << acc;
-      pend_parity = (pend_parity & ~(1u << acc)) | (aphase << acc);
-      if (++acc == 2u) {
-        acc = 0;
-        aphase ^= 1u;
+        if (in_seg == C::SEG - 1u || st + 1u == st1) {
+          tc::mma_commit_elect(&sh.tfull[acc]);
+          pending |= 1u << acc;
+          pend_parity = (pend_parity & ~(1u << acc)) | (aphase << acc);
+          if (++acc == NACC) {
+            acc = 0;
+            aphase ^= 1u;
+          }
+        }
       }
     }
     // every MMA is complete before the columns are freed
-    for (uint32_t i = 0; i < 2; ++i)
+    for (uint32_t i = 0; i < NACC; ++i)
       if (pending & (1u << i))
         if (!mbar_wait(&sh.tfull[i], (pend_parity >> i) & 1u)) raise_flag(a.flags, PW_FLAG_WAIT_TIMEOUT);
   } else {
     // two warps per TMEM lane quarter, each half of the token columns (all of
     // them for the first when there are only 32)
     const uint32_t quarter = warp % 4u, half = (warp - kEpiWarp0) / 4u;
-    constexpr uint32_t COLS = BN >= 64 ? BN / 2 : 32;
+    constexpr uint32_t COLS = BN >= 64 ? BN / 2 : 32, CH = COLS / 32u;
     const uint32_t col0 = half * COLS;
+    const bool active = col0 < (uint32_t)BN;
+    const uint32_t row = quarter * 32u + lane;  // of the tile
     uint32_t acc = 0, aphase = 0;
-    for (uint32_t u = blockIdx.x; u < total; u += gridDim.x) {
+    for (uint32_t u = u_begin; u < total; u += u_step) {
       uint32_t rt, tt;
       tile_of(A, u, rt, tt);
-      const uint32_t c = rt * kTileRows + quarter * 32u + lane;
+      const uint32_t c = rt * kTileRows + row, tok0 = tt * BN;
       const bool mine = c < a.rows;
       const float bias = mine && a.ep.bias ? load_elem(a.ep.bias, c, a.ep.bias_dtype) : 0.0f;
-      const bool ok = lwait(sh, &sh.tfull[acc], aphase, a.flags);
-      tc_fence_after();
-      const uint32_t src = tmem + ((quarter * 32u) << 16) + acc * (uint32_t)BN + col0;
-      if (ok && col0 < (uint32_t)BN) {
-        for (uint32_t q = 0; q < COLS; q += 32u) {
-          float v[32];
-          tc::tmem_ld32(src + q, v);
-          tc::tmem_wait_ld(v);
-          const uint32_t t0 = tt * BN + col0 + q;
-          if (mine && t0 < a.width) finish32(a.ep, v, bias, t0, c, min(32u, a.width - t0), a.flags);
-          __syncwarp();
+      float sum[CH][32];
+#pragma unroll
+      for (uint32_t q = 0; q < CH; ++q)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) sum[q][j] = 0.0f;
+      for (uint32_t st = st0; st < st1; st += C::SEG) {
+        const bool ok = __all_sync(0xffffffffu, lwait(sh, &sh.tfull[acc], aphase, a.flags));
+        tc_fence_after();
+        if (ok && active) {
+          const uint32_t src = tmem + ((quarter * 32u) << 16) + acc * (uint32_t)BN + col0;
+#pragma unroll
+          for (uint32_t q = 0; q < CH; ++q) {
+            float v[32];
+            tc::tmem_ld32(src + 32u * q, v);
+            tc::tmem_wait_ld(v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[q][j] += v[j];
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.tempty[acc]);
+        if (++acc == NACC) {
+          acc = 0;
+          aphase ^= 1u;
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.tempty[acc]);
-      if (++acc == 2u) {
-        acc = 0;
-        aphase ^= 1u;
+      if (splits == 1u) {
+        if (active && mine)
+#pragma unroll
+          for (uint32_t q = 0; q < CH; ++q) {
+            const uint32_t t0 = tok0 + col0 + 32u * q;
+            if (t0 < a.width) {
+              const uint32_t n = min(32u, a.width - t0);
+              uint32_t raw[32];
+              if (a.ep.residual) load_residual32(a.ep, t0, c, n, raw);
+              finish32(a.ep, sum[q], bias, raw, t0, c, n, a.flags);
+            }
+          }
+      } else {
+        // CTA k of the cluster finishes tokens [k * share, (k + 1) * share) of the
+        // tile: send it their sums, [rank][token][row] in its ring
+        const uint32_t tokens = min((uint32_t)BN, a.width - tok0), share = (tokens + splits - 1u) / splits;
+        __syncwarp();
+        cluster_sync_all();  // every CTA's MMAs have read their last stage
+        if (active) {
+          const uint32_t mine_at = smem_addr(sh.ring) + (rank * share * kTileRows + row) * 4u;
+          uint32_t to = col0 / share, at = col0 % share;  // of token col0 + 32 q + j
+          uint32_t dst = map_rank(mine_at, to < splits ? to : 0u) + at * (kTileRows * 4u);
+#pragma unroll
+          for (uint32_t q = 0; q < CH; ++q)
+#pragma unroll
+            for (uint32_t j = 0; j < 32; ++j)
+              if (col0 + 32u * q + j < tokens) {
+                store_remote(dst, sum[q][j]);
+                dst += kTileRows * 4u;
+                if (++at == share) {
+                  at = 0;
+                  if (++to < splits) dst = map_rank(mine_at, to);
+                }
+              }
+        }
+        __syncwarp();
+        cluster_sync_all();
+        const float *got = reinterpret_cast<const float *>(sh.ring);
+        const uint32_t first = rank * share, n = first < tokens ? min(share, tokens - first) : 0u;
+        if (mine)
+          for (uint32_t i = half; i < n; i += 2u) {
+            float v = got[i * kTileRows + row];
+            for (uint32_t s = 1; s < splits; ++s) v += got[(s * share + i) * kTileRows + row];
+            const uint64_t t = tok0 + first + i;
+            if (!store_elem(a.ep.y, t * a.ep.y_stride + c, a.ep.y_dtype, epilogue_value(a.ep, v, t, c)))
+              raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
+          }
       }
     }
+  }
+  if (splits > 1u && warp < (uint32_t)kEpiWarp0) {
+    // the epilogue's two cluster barriers count every thread
+    __syncwarp();
+    cluster_sync_all();
+    cluster_sync_all();
   }
 
   tc_fence_before();
@@ -306,26 +505,228 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tc(const __grid_constant
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
 }
 
-template <int BN>
-cudaError_t launch_tc(const LinearArgs &a, int num_sms, cudaStream_t stream) {
-  using C = Cfg<BN>;
-  Args A{};
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linear_pair(const __grid_constant__ Args A) {
+  using C = PairCfg;
+  constexpr uint32_t NST = C::NST, BN = C::BN;
+  const LinearArgs &a = A.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Shared sh;
+  sh.ring = smem;
+  sh.full = reinterpret_cast<uint64_t *>(smem + C::BARS);
+  sh.empty = sh.full + NST;
+  sh.tfull = sh.empty + NST;
+  sh.tempty = sh.tfull + 2;
+  sh.tmem_base = reinterpret_cast<uint32_t *>(smem + C::MISC);
+  sh.abort = reinterpret_cast<volatile int *>(smem + C::MISC + 4);
+
+  const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = cluster_rank();
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < NST; ++i) {
+      mbar_init(&sh.full[i], 1);   // the leading CTA's: both CTAs' loads complete on it
+      mbar_init(&sh.empty[i], 1);  // each CTA's: the pair's commit after the stage's MMAs
+    }
+    for (uint32_t i = 0; i < 2; ++i) {
+      mbar_init(&sh.tfull[i], 1);                // each CTA's: the pair's commit after the tile's MMAs
+      mbar_init(&sh.tempty[i], 2u * kEpiWarps);  // the leading CTA's: both CTAs' epilogue warps
+    }
+    *sh.abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == (uint32_t)kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(sh.tmem_base)),
+                 "r"(C::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  cluster_sync_all();  // both CTAs' barriers are initialised
+  tc_fence_after();
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t tmem = *sh.tmem_base;
+  const uint32_t total = A.row_tiles * A.token_tiles, u_begin = blockIdx.x / 2u, u_step = gridDim.x / 2u;
+
+  if (warp == (uint32_t)kProducerWarp) {
+    // this CTA's 128 weight rows and its half of the tokens
+    uint32_t slot = 0, phase = 0, issued = 0, parity = 0;
+    for (uint32_t u = u_begin; u < total; u += u_step) {
+      uint32_t rt, tt;
+      tile_of(A, u, rt, tt);
+      const int row0 = (int)(rt * 2u * kTileRows + rank * kTileRows), tok0 = (int)(tt * BN + rank * (BN / 2u));
+      for (uint32_t kb = 0; kb < A.stages; ++kb) {
+        if (lwait(sh, &sh.empty[slot], phase ^ 1u, a.flags)) {
+          uint8_t *dst = sh.ring + slot * C::STAGE;
+          if (elect_one()) {
+            const uint32_t bar = map_rank(smem_addr(&sh.full[slot]), 0u);
+            if (rank == 0u) mbar_arrive_expect_tx(&sh.full[slot], 2u * C::STAGE);
+            if (A.k3d) {
+              tma_load_pair(dst, &A.wmap, 0, row0, (int)kb, bar);
+              tma_load_pair(dst + C::A_BYTES, &A.xmap, 0, tok0, (int)kb, bar);
+            } else {
+              tma_load_pair(dst, &A.wmap, (int)(kb * kBlockK), row0, 0, bar);
+              tma_load_pair(dst + C::A_BYTES, &A.xmap, (int)(kb * kBlockK), tok0, 0, bar);
+            }
+          }
+          __syncwarp();
+          issued |= 1u << slot;
+          parity = (parity & ~(1u << slot)) | (phase << slot);
+        }
+        if (++slot == NST) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    // every copy in flight lands before either CTA can exit
+    if (rank == 0u)
+      for (uint32_t i = 0; i < NST; ++i)
+        if (issued & (1u << i))
+          if (!mbar_wait(&sh.full[i], (parity >> i) & 1u)) raise_flag(a.flags, PW_FLAG_WAIT_TIMEOUT);
+  } else if (warp == (uint32_t)kMmaWarp) {
+    if (rank == 0u) {
+      const uint32_t idesc = instr_desc16(BN, 2u * kTileRows, a.dtype == PW_DTYPE_BF16);
+      const uint64_t ring_desc = smem_desc_sw128(smem_addr(sh.ring));
+      uint32_t slot = 0, phase = 0, acc = 0, aphase = 0, pending = 0, pend_parity = 0;
+      for (uint32_t u = u_begin; u < total; u += u_step) {
+        const bool ok_acc = lwait<true>(sh, &sh.tempty[acc], aphase ^ 1u, a.flags);
+        tc_fence_after();
+        const uint32_t d = tmem + acc * BN;
+        for (uint32_t kb = 0; kb < A.stages; ++kb) {
+          const bool ok = lwait(sh, &sh.full[slot], phase, a.flags) && ok_acc;
+          tc_fence_after();
+          if (ok) {
+            const uint64_t ad = ring_desc + ((slot * C::STAGE) >> 4);
+            const uint64_t bd = ad + (C::A_BYTES >> 4);
+#pragma unroll
+            for (uint32_t s = 0; s < 4; ++s)
+              mma_f16_pair_elect(d, ad + 2u * s, bd + 2u * s, idesc, (kb | s) ? 1u : 0u);
+          }
+          mma_commit_pair_elect(&sh.empty[slot]);
+          if (++slot == NST) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+        mma_commit_pair_elect(&sh.tfull[acc]);
+        pending |= 1u << acc;
+        pend_parity = (pend_parity & ~(1u << acc)) | (aphase << acc);
+        if (++acc == 2u) {
+          acc = 0;
+          aphase ^= 1u;
+        }
+      }
+      // every MMA is complete before either CTA's columns are freed
+      for (uint32_t i = 0; i < 2; ++i)
+        if (pending & (1u << i))
+          if (!mbar_wait(&sh.tfull[i], (pend_parity >> i) & 1u)) raise_flag(a.flags, PW_FLAG_WAIT_TIMEOUT);
+    }
+  } else {
+    // this CTA's 128 rows: two warps per TMEM lane quarter, half of the tokens each
+    const uint32_t quarter = warp % 4u, half = (warp - kEpiWarp0) / 4u, col0 = half * (BN / 2u);
+    uint32_t acc = 0, aphase = 0;
+    for (uint32_t u = u_begin; u < total; u += u_step) {
+      uint32_t rt, tt;
+      tile_of(A, u, rt, tt);
+      const uint32_t c = rt * 2u * kTileRows + rank * kTileRows + quarter * 32u + lane;
+      const bool mine = c < a.rows;
+      const float bias = mine && a.ep.bias ? load_elem(a.ep.bias, c, a.ep.bias_dtype) : 0.0f;
+      // 32 tokens at a time, their residual loaded one step ahead (the first
+      // while the tile's products still run)
+      const uint32_t t_begin = tt * BN + col0;
+      const bool add = mine && a.ep.residual != nullptr;
+      uint32_t raw[32];
+      if (add && t_begin < a.width) load_residual32(a.ep, t_begin, c, min(32u, a.width - t_begin), raw);
+      const bool ok = __all_sync(0xffffffffu, lwait(sh, &sh.tfull[acc], aphase, a.flags));
+      tc_fence_after();
+      const uint32_t src = tmem + ((quarter * 32u) << 16) + acc * BN + col0;
+      if (ok) {
+#pragma unroll 1
+        for (uint32_t q = 0; q < BN / 2u; q += 32u) {
+          float v[32];
+          tc::tmem_ld32(src + q, v);
+          tc::tmem_wait_ld(v);
+          const uint32_t t0 = t_begin + q, t1 = t0 + 32u;
+          uint32_t cur[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) cur[j] = raw[j];
+          if (add && q + 32u < BN / 2u && t1 < a.width) load_residual32(a.ep, t1, c, min(32u, a.width - t1), raw);
+          if (mine && t0 < a.width) finish32(a.ep, v, bias, cur, t0, c, min(32u, a.width - t0), a.flags);
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_remote(map_rank(smem_addr(&sh.tempty[acc]), 0u));
+      if (++acc == 2u) {
+        acc = 0;
+        aphase ^= 1u;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  cluster_sync_all();  // neither CTA's shared memory or columns go before both are done
+  tc_fence_after();
+  if (warp == (uint32_t)kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
+}
+
+// The kernel's arguments over tiles of `rows` x `tokens`, boxes of `box_tokens`
+// tokens and `kbs` k-blocks per stage; false when a map cannot be made.
+bool make_args(const LinearArgs &a, uint32_t rows, uint32_t tokens, uint32_t box_tokens, uint32_t kbs, Args &A) {
   A.a = a;
-  A.w3d = a.cols % kBlockK == 0u;
-  A.x3d = A.w3d;
-  const uint32_t kb = A.w3d ? C::KBS : 0u;
+  A.k3d = a.cols % kBlockK == 0u;
+  const uint32_t kb = A.k3d ? kbs : 0u;
   if (!encode_rows16_map(&A.wmap, a.w, a.rows, a.cols, a.w_stride, a.dtype, kTileRows, kb) ||
-      !encode_rows16_map(&A.xmap, a.x, a.width, a.cols, a.x_stride, a.dtype, BN, kb))
-    return cudaErrorInvalidValue;
-  A.row_tiles = (a.rows + kTileRows - 1u) / kTileRows;
-  A.token_tiles = (a.width + (uint32_t)BN - 1u) / (uint32_t)BN;
-  A.stages = (a.cols + C::KBS * kBlockK - 1u) / (C::KBS * kBlockK);
-  cudaError_t e = allow_smem<k_linear_tc<BN>>(C::SMEM);
+      !encode_rows16_map(&A.xmap, a.x, a.width, a.cols, a.x_stride, a.dtype, box_tokens, kb))
+    return false;
+  A.row_tiles = (a.rows + rows - 1u) / rows;
+  A.token_tiles = (a.width + tokens - 1u) / tokens;
+  A.stages = (a.cols + kbs * kBlockK - 1u) / (kbs * kBlockK);
+  A.splits = 1u;
+  return (uint64_t)A.row_tiles * A.token_tiles <= 0x7fffffffull / kMaxSplits;
+}
+
+template <int BN>
+cudaError_t launch_tile(const LinearArgs &a, uint32_t splits, int num_sms, cudaStream_t stream) {
+  using C = TileCfg<BN>;
+  Args A{};
+  if (!make_args(a, kTileRows, BN, BN, C::KBS, A)) return cudaErrorInvalidValue;
+  cudaError_t e = allow_smem<k_linear_tile<BN>>(C::SMEM);
   if (e != cudaSuccess) return e;
-  const uint64_t tiles = (uint64_t)A.row_tiles * A.token_tiles;
-  if (tiles > 0x7fffffffull) return cudaErrorInvalidValue;
-  const uint32_t grid = tiles < (uint64_t)num_sms ? (uint32_t)tiles : (uint32_t)num_sms;
-  return launch_kernel(k_linear_tc<BN>, dim3(grid), dim3(kThreads), C::SMEM, stream, A);
+  A.splits = splits;
+  const uint32_t tiles = A.row_tiles * A.token_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(splits > 1u ? tiles * splits : tiles < (uint32_t)num_sms ? tiles : (uint32_t)num_sms);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1u ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, k_linear_tile<BN>, A);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+cudaError_t launch_pair(const LinearArgs &a, int num_sms, cudaStream_t stream) {
+  using C = PairCfg;
+  Args A{};
+  if (!make_args(a, 2u * kTileRows, C::BN, C::BN / 2u, 1u, A)) return cudaErrorInvalidValue;
+  cudaError_t e = allow_smem<k_linear_pair>(C::SMEM);
+  if (e != cudaSuccess) return e;
+  const uint32_t tiles = A.row_tiles * A.token_tiles, pairs = (uint32_t)num_sms / 2u;
+  return launch_kernel(k_linear_pair, dim3(2u * (tiles < pairs ? tiles : pairs)), dim3(kThreads), C::SMEM, stream, A);
 }
 
 // ------------------------------------------------------------- row conversion
@@ -355,11 +756,25 @@ cudaError_t launch_convert_rows(const void *x, uint64_t x_stride, uint32_t x_dty
 cudaError_t launch_linear(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   if (a.rows == 0 || a.cols == 0 || (a.dtype != PW_DTYPE_BF16 && a.dtype != PW_DTYPE_F16)) return cudaErrorInvalidValue;
   if (a.width == 0) return cudaSuccess;
-  if (a.width <= 16u && !getenv("PW_NONARROW")) return launch_linear_narrow(a, num_sms, stream);
-  if (a.width <= 32u) return lin::launch_tc<32>(a, num_sms, stream);
-  if (a.width <= 64u) return lin::launch_tc<64>(a, num_sms, stream);
-  if (a.width <= 128u) return lin::launch_tc<128>(a, num_sms, stream);
-  return lin::launch_tc<256>(a, num_sms, stream);
+  if (a.width <= 16u) return launch_linear_narrow(a, num_sms, stream);
+  // Tiles of one CTA: as many K splits as fill the SMs, each of two stages or more.
+  const uint64_t sms = (uint64_t)num_sms;
+  const uint32_t bn = a.width <= 32u ? 32u : a.width <= 64u ? 64u : 128u;
+  const uint64_t tiles = (uint64_t)((a.rows + lin::kTileRows - 1u) / lin::kTileRows) * ((a.width + bn - 1u) / bn);
+  const uint32_t stages = (a.cols + 2u * lin::kBlockK - 1u) / (2u * lin::kBlockK);
+  uint64_t splits = sms / (tiles ? tiles : 1u);
+  splits = splits > stages / 2u ? stages / 2u : splits;
+  splits = splits > lin::kMaxSplits ? lin::kMaxSplits : splits < 1u ? 1u : splits;
+  // Pairs do two such tiles' work per CTA and tile, at about 1.5 times the rate
+  // (shared memory feeds the 128 x 128 tile's products at 2/3 of the tensor
+  // rate), but cannot split K.
+  const uint64_t pair_tiles = (uint64_t)((a.rows + 255u) / 256u) * ((a.width + 255u) / 256u);
+  const double pair_cost = (double)((pair_tiles + sms / 2u - 1u) / (sms / 2u)) * 2.0;
+  const double tile_cost = (double)((tiles * splits + sms - 1u) / sms) / (double)splits * 1.5;
+  if (a.ep.y_dtype != PW_DTYPE_F32 && a.width > 128u && pair_cost <= tile_cost) return lin::launch_pair(a, num_sms, stream);
+  if (bn == 32u) return lin::launch_tile<32>(a, (uint32_t)splits, num_sms, stream);
+  if (bn == 64u) return lin::launch_tile<64>(a, (uint32_t)splits, num_sms, stream);
+  return lin::launch_tile<128>(a, (uint32_t)splits, num_sms, stream);
 }
 
 }  // namespace pw

@@ -236,6 +236,32 @@ def test_linear_sums_are_exact_on_small_integers(rt, width, rows, cols, dtype):
     assert (buf[:, rows:] == 9.0).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("width,rows,cols", [(1500, 2600, 64), (700, 4100, 72), (1500, 3001, 1003), (1030, 5130, 456),
+                                             (2048, 4096, 1856), (129, 9500, 128)])
+def test_wide_linear_sums_are_exact_on_small_integers(rt, width, rows, cols, dtype):
+    # sums of products of -1, 0 and 1 stay below 2048: exact in f16 too
+    t = TYPES[dtype]
+    x, _ = wide(torch.randint(-1, 2, (width, cols), generator=gen(31), device="cuda").to(t), -cols % 8 + 8, float("nan"))
+    w, _ = wide(torch.randint(-1, 2, (rows, cols), generator=gen(32), device="cuda").to(t), -cols % 8, float("nan"))
+    out, buf = wide(torch.zeros((width, rows), device="cuda", dtype=torch.float16), 3, 9.0)
+    rt.linear(x, w, out=out)
+    assert torch.equal(out.float(), x.float() @ w.float().t())
+    assert (buf[:, rows:] == 9.0).all()
+
+
+@pytest.mark.parametrize("width,rows,cols", [(40, 300, 4096), (64, 1000, 1000), (100, 4096, 8192), (77, 5001, 1003),
+                                             (200, 130, 16384), (300, 512, 640)])
+def test_linear_f32_keeps_its_digits(rt, width, rows, cols):
+    # sums in segments of at most 512 columns (32 steps, 2^-23 each at worst), joined in f32: the relative error of
+    # the whole output stays below 32 2^-23 and the joins' K / 512 2^-24
+    x, w = randn((width, cols), 33, torch.bfloat16), randn((rows, cols), 34, torch.bfloat16, cols ** -0.5)
+    w, _ = wide(w, -cols % 8)
+    ref = x.double() @ w.double().t()
+    got = rt.linear(x, w, out_dtype=torch.float32).output.double()
+    assert ((got - ref).norm() / ref.norm()).item() <= 32 * 2.0 ** -23 + cols / 512 * 2.0 ** -24
+
+
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("width,rows,cols", [(1, 520, 1024), (5, 130, 200), (40, 257, 512), (200, 300, 776),
                                              (520, 260, 1024)])
