@@ -12,17 +12,21 @@
 //  * k_linear_pair, for many tokens and 16-bit outputs: two CTAs on one 256 x 256
 //    tile (cta_group::2): each holds its 128 weight rows and half of the tokens,
 //    so the shared memory that a tensor core reads per product is half of what a
-//    128 x 256 tile of one CTA needs.  Persistent pairs, two accumulators, the
-//    whole K in one accumulator.  Bound by the tensor pipe.
+//    128 x 256 tile of one CTA needs.  Persistent pairs, two accumulators, all of
+//    a tile's K in one accumulator.  Bound by the tensor pipe.
 //  * k_linear_tile, for the widths between and for f32 outputs: 128 x 32, 64 or
 //    128 tiles of one CTA.  K runs in segments of 512 columns: each gets a fresh
 //    accumulator, and the epilogue adds the segments in registers.  (The tensor
 //    pipe truncates when it adds to an accumulator: over 4096 columns in one
 //    accumulator an f32 result was 4.4e-6 off, with segments it is below 1e-6; a
-//    16-bit result does not show it.)  When the tiles are fewer than the SMs, the
-//    CTAs of a cluster split K and exchange their sums through distributed shared
-//    memory, each finishing its share of the tokens: HBM bounds these widths, and
-//    a stream over a third of the SMs does not reach it.
+//    16-bit result does not show it.)
+//
+// When the tiles are fewer than the SMs, the CTAs (pairs) of a cluster split K:
+// HBM bounds these widths, and a stream over a third of the SMs does not reach
+// it.  They exchange their sums through distributed shared memory, 16 bytes per
+// store, and each finishes its share of the tokens, so the join is as parallel as
+// the products (77 x 5000 x 1024: 12.7 us when each lane sent single values and
+// joined token by token, - us so).
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -66,7 +70,7 @@ struct TileCfg {
   static constexpr uint32_t TMEM_COLS = NACC * (uint32_t)BN;
   static_assert(SMEM <= kSmemLimit, "shared memory");
   // the K splits' exchange reuses the ring: [split][token of the share][128 rows] f32
-  static_assert(((uint32_t)BN + kMaxSplits) * kTileRows * 4u <= NST * STAGE, "exchange buffer");
+  static_assert(((uint32_t)BN + 8u * kMaxSplits) * kTileRows * 4u <= NST * STAGE, "exchange buffer");
 };
 
 struct PairCfg {
@@ -80,6 +84,7 @@ struct PairCfg {
   static constexpr uint32_t SMEM = MISC + 16u + 1024u;
   static constexpr uint32_t TMEM_COLS = 2u * BN;
   static_assert(SMEM <= kSmemLimit, "shared memory");
+  static_assert((BN + 8u * kMaxSplits) * kTileRows * 4u <= NST * STAGE, "exchange buffer");
 };
 
 struct Args {
@@ -117,13 +122,13 @@ __device__ __forceinline__ void mma_f16_pair_elect(uint32_t d, uint64_t a, uint6
       : "memory");
 }
 // Arrives on the barrier at this offset in both CTAs once the MMAs so far are complete.
-__device__ __forceinline__ void mma_commit_pair_elect(uint64_t *bar) {
+__device__ __forceinline__ void mma_commit_pair_elect(uint64_t *bar, uint32_t pair_mask) {
   asm volatile(
       "{\n\t.reg .pred e;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
           smem_addr(bar)),
-      "h"((uint16_t)3)
+      "h"((uint16_t)pair_mask)
       : "memory");
 }
 // A tile load into this CTA's shared memory that completes on the pair's
@@ -150,11 +155,15 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void store_remote(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+__device__ __forceinline__ void store_remote4(uint32_t addr, float x, float y, float z, float w) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
 }
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
 struct Shared {
@@ -213,59 +222,138 @@ __device__ __forceinline__ void tile_of(const Args &A, uint32_t u, uint32_t &row
 }
 
 // The residual of output column c, tokens t0 .. t0 + n - 1 (n >= 1): loads only,
-// all 32 in flight, so they can be issued before what they are added to is ready.
+// all N in flight, so they can be issued before what they are added to is ready.
 // Past the last token they repeat it.
-__device__ __forceinline__ void load_residual32(const EpilogueArgs &e, uint64_t t0, uint32_t c, uint32_t n,
-                                                uint32_t (&raw)[32]) {
+template <int N>
+__device__ __forceinline__ void load_residual(const EpilogueArgs &e, uint64_t t0, uint32_t c, uint32_t n,
+                                              uint32_t (&raw)[N]) {
   const uint64_t at = t0 * e.residual_stride + c;
   if (e.residual_dtype == PW_DTYPE_F32) {
     const uint32_t *p = static_cast<const uint32_t *>(e.residual) + at;
 #pragma unroll
-    for (uint32_t j = 0; j < 32; ++j) raw[j] = p[min(j, n - 1u) * e.residual_stride];
+    for (uint32_t j = 0; j < N; ++j) raw[j] = p[min(j, n - 1u) * e.residual_stride];
   } else {
     const uint16_t *p = static_cast<const uint16_t *>(e.residual) + at;
 #pragma unroll
-    for (uint32_t j = 0; j < 32; ++j) raw[j] = p[min(j, n - 1u) * e.residual_stride];
+    for (uint32_t j = 0; j < N; ++j) raw[j] = p[min(j, n - 1u) * e.residual_stride];
   }
 }
 
-__device__ __forceinline__ void add_residual32(const EpilogueArgs &e, const uint32_t (&raw)[32], float (&v)[32]) {
-  if (e.residual_dtype == PW_DTYPE_F32) {
+template <typename T, int N>
+__device__ __forceinline__ void store_rows(const float (&v)[N], T *p, uint64_t stride, uint32_t n) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(raw[j]);
-  } else if (e.residual_dtype == PW_DTYPE_BF16) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(raw[j] << 16);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] += __half2float(__ushort_as_half((unsigned short)raw[j]));
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void store_rows(const float (&v)[32], T *p, uint64_t stride, uint32_t n) {
-#pragma unroll
-  for (uint32_t j = 0; j < 32; ++j)
+  for (uint32_t j = 0; j < N; ++j)
     if (j < n) p[j * stride] = from_f32<T>(v[j]);
 }
 
 // The epilogue of one thread: output column c of tokens t0 .. t0 + n - 1, raw its
-// residual (load_residual32).
-__device__ __forceinline__ void finish32(const EpilogueArgs &e, float (&v)[32], float bias, const uint32_t (&raw)[32],
-                                         uint64_t t0, uint32_t c, uint32_t n, uint32_t *flags) {
+// residual (load_residual).
+template <int N>
+__device__ __forceinline__ void finish(const EpilogueArgs &e, float (&v)[N], float bias, const uint32_t (&raw)[N],
+                                       uint64_t t0, uint32_t c, uint32_t n, uint32_t *flags) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] += bias;
+  for (int j = 0; j < N; ++j) v[j] += bias;
   activate_all(v, e.act);
-  if (e.residual) add_residual32(e, raw, v);
+  if (e.residual) {
+    if (e.residual_dtype == PW_DTYPE_F32) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] += __uint_as_float(raw[j]);
+    } else if (e.residual_dtype == PW_DTYPE_BF16) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] += __uint_as_float(raw[j] << 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] += __half2float(__ushort_as_half((unsigned short)raw[j]));
+    }
+  }
   uint32_t top = 0u;
 #pragma unroll
-  for (uint32_t j = 0; j < 32; ++j)
+  for (uint32_t j = 0; j < N; ++j)
     if (j < n) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
   if (top >= overflow_bits(e.y_dtype)) raise_flag(flags, PW_FLAG_NONFINITE_ROUND);
   const uint64_t at = t0 * e.y_stride + c;
   if (e.y_dtype == PW_DTYPE_F32) store_rows(v, static_cast<float *>(e.y) + at, e.y_stride, n);
   else if (e.y_dtype == PW_DTYPE_BF16) store_rows(v, static_cast<__nv_bfloat16 *>(e.y) + at, e.y_stride, n);
   else store_rows(v, static_cast<__half *>(e.y) + at, e.y_stride, n);
+}
+
+// Joining K splits.  Split k of a tile finishes tokens [k share, (k + 1) share) of
+// the tile's `tokens`; share is a multiple of 8, so that a quad of tokens has one
+// owner and each half of the epilogue warps whole quads.  The sums travel as
+// [source split][quad of the share][128 rows][4 tokens] f32.
+struct Exchange {
+  uint32_t ring;    // this CTA's ring
+  uint32_t splits, split, step, base;  // split k is the cluster's CTA base + step k
+  uint32_t tokens, share;
+  __device__ __forceinline__ Exchange(uint8_t *r, uint32_t n_splits, uint32_t k, uint32_t cta_step, uint32_t cta_base,
+                                      uint32_t n_tokens)
+      : ring(smem_addr(r)), splits(n_splits), split(k), step(cta_step), base(cta_base), tokens(n_tokens) {
+    share = ((n_tokens + n_splits - 1u) / n_splits + 7u) & ~7u;
+  }
+  __device__ __forceinline__ uint32_t slot(uint32_t from, uint32_t token_of_share, uint32_t row) const {
+    return ((from * (share / 4u) + token_of_share / 4u) * kTileRows + row) * 16u;
+  }
+  // this row's sums of tile tokens t0 .. t0 + 31 (t0 % 32 == 0) to their owners
+  __device__ __forceinline__ void send32(const float (&v)[32], uint32_t t0, uint32_t row) const {
+    uint32_t to = t0 / share, at = t0 % share;
+    uint32_t dst = to < splits ? map_rank(ring + slot(split, 0u, row), base + step * to) : 0u;
+#pragma unroll
+    for (uint32_t q = 0; q < 8; ++q) {
+      if (t0 + 4u * q < tokens) store_remote4(dst + slot(0u, at, 0u), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      at += 4u;
+      if (at == share && to + 1u < splits) {
+        at = 0u;
+        ++to;
+        dst = map_rank(ring + slot(split, 0u, row), base + step * to);
+      }
+    }
+  }
+  // this row's joined sums of tokens b .. b + 7 of this CTA's share
+  __device__ __forceinline__ void receive8(float (&v)[8], uint32_t b, uint32_t row) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    for (uint32_t s = 0; s < splits; ++s)
+#pragma unroll
+      for (uint32_t q = 0; q < 2; ++q) {
+        float x, y, z, w;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(x), "=f"(y), "=f"(z), "=f"(w)
+                     : "r"(ring + slot(s, b + 4u * q, row)));
+        v[4 * q] += x;
+        v[4 * q + 1] += y;
+        v[4 * q + 2] += z;
+        v[4 * q + 3] += w;
+      }
+  }
+};
+
+// The rest of a split tile's epilogue, from the CTA's own sums sent: joins and
+// finishes this thread's row (output column c) for its half of the share, 8
+// tokens at a time (each CTA runs this once: a short loop, because code that is
+// fetched for the first time costs more than it computes).
+__device__ __forceinline__ void finish_share(const Exchange &x, const LinearArgs &a, float bias, uint32_t tok0,
+                                             uint32_t c, uint32_t row, uint32_t half) {
+  const bool mine = c < a.rows;
+  const uint32_t first = x.split * x.share, mid = x.share / 2u & ~7u;
+  // tokens [begin, end) of the share
+  const uint32_t in_tile = first < x.tokens ? min(x.share, x.tokens - first) : 0u;
+  const uint32_t begin = half ? mid : 0u, end = half ? in_tile : min(mid, in_tile);
+  uint32_t raw[8];
+  const bool add = mine && a.ep.residual != nullptr;
+  if (add && begin < end) load_residual(a.ep, tok0 + first + begin, c, min(8u, end - begin), raw);
+  __syncwarp();
+  cluster_sync_all();  // every CTA's sums have arrived
+#pragma unroll 1
+  for (uint32_t b = begin; b < end; b += 8u) {
+    const uint32_t n = min(8u, end - b);
+    uint32_t cur[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) cur[j] = raw[j];
+    if (add && b + 8u < end) load_residual(a.ep, tok0 + first + b + 8u, c, min(8u, end - b - 8u), raw);
+    float v[8];
+    x.receive8(v, b, row);
+    if (mine) finish(a.ep, v, bias, cur, tok0 + first + b, c, n, a.flags);
+  }
 }
 
 template <int BN>
@@ -296,6 +384,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tile(const __grid_consta
     }
     *sh.abort = 0;
     mbar_fence_init();
+  }
+  if (warp == (uint32_t)kProducerWarp && elect_one()) {
+    prefetch_map(&A.wmap);
+    prefetch_map(&A.xmap);
   }
   if (warp == (uint32_t)kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(sh.tmem_base)),
@@ -449,45 +541,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tile(const __grid_consta
             if (t0 < a.width) {
               const uint32_t n = min(32u, a.width - t0);
               uint32_t raw[32];
-              if (a.ep.residual) load_residual32(a.ep, t0, c, n, raw);
-              finish32(a.ep, sum[q], bias, raw, t0, c, n, a.flags);
+              if (a.ep.residual) load_residual(a.ep, t0, c, n, raw);
+              finish(a.ep, sum[q], bias, raw, t0, c, n, a.flags);
             }
           }
       } else {
-        // CTA k of the cluster finishes tokens [k * share, (k + 1) * share) of the
-        // tile: send it their sums, [rank][token][row] in its ring
-        const uint32_t tokens = min((uint32_t)BN, a.width - tok0), share = (tokens + splits - 1u) / splits;
+        const Exchange x(sh.ring, splits, rank, 1u, 0u, min((uint32_t)BN, a.width - tok0));
         __syncwarp();
         cluster_sync_all();  // every CTA's MMAs have read their last stage
-        if (active) {
-          const uint32_t mine_at = smem_addr(sh.ring) + (rank * share * kTileRows + row) * 4u;
-          uint32_t to = col0 / share, at = col0 % share;  // of token col0 + 32 q + j
-          uint32_t dst = map_rank(mine_at, to < splits ? to : 0u) + at * (kTileRows * 4u);
+        if (active)
 #pragma unroll
-          for (uint32_t q = 0; q < CH; ++q)
-#pragma unroll
-            for (uint32_t j = 0; j < 32; ++j)
-              if (col0 + 32u * q + j < tokens) {
-                store_remote(dst, sum[q][j]);
-                dst += kTileRows * 4u;
-                if (++at == share) {
-                  at = 0;
-                  if (++to < splits) dst = map_rank(mine_at, to);
-                }
-              }
-        }
-        __syncwarp();
-        cluster_sync_all();
-        const float *got = reinterpret_cast<const float *>(sh.ring);
-        const uint32_t first = rank * share, n = first < tokens ? min(share, tokens - first) : 0u;
-        if (mine)
-          for (uint32_t i = half; i < n; i += 2u) {
-            float v = got[i * kTileRows + row];
-            for (uint32_t s = 1; s < splits; ++s) v += got[(s * share + i) * kTileRows + row];
-            const uint64_t t = tok0 + first + i;
-            if (!store_elem(a.ep.y, t * a.ep.y_stride + c, a.ep.y_dtype, epilogue_value(a.ep, v, t, c)))
-              raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
-          }
+          for (uint32_t q = 0; q < CH; ++q) x.send32(sum[q], col0 + 32u * q, row);
+        finish_share(x, a, bias, tok0, c, row, half);
       }
     }
   }
@@ -505,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tile(const __grid_consta
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linear_pair(const __grid_constant__ Args A) {
+__global__ void __launch_bounds__(kThreads, 1) k_linear_pair(const __grid_constant__ Args A) {
   using C = PairCfg;
   constexpr uint32_t NST = C::NST, BN = C::BN;
   const LinearArgs &a = A.a;
@@ -520,7 +585,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linea
   sh.tmem_base = reinterpret_cast<uint32_t *>(smem + C::MISC);
   sh.abort = reinterpret_cast<volatile int *>(smem + C::MISC + 4);
 
-  const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = cluster_rank();
+  const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+  // cluster CTAs 2 k and 2 k + 1 are the pair of K split k
+  const uint32_t cta = cluster_rank(), rank = cta & 1u, lead = cta & ~1u;
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < NST; ++i) {
       mbar_init(&sh.full[i], 1);   // the leading CTA's: both CTAs' loads complete on it
@@ -532,6 +599,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linea
     }
     *sh.abort = 0;
     mbar_fence_init();
+  }
+  if (warp == (uint32_t)kProducerWarp && elect_one()) {
+    prefetch_map(&A.wmap);
+    prefetch_map(&A.xmap);
   }
   if (warp == (uint32_t)kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(sh.tmem_base)),
@@ -547,7 +618,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linea
   pdl_wait();
   pdl_launch_dependents();
   const uint32_t tmem = *sh.tmem_base;
-  const uint32_t total = A.row_tiles * A.token_tiles, u_begin = blockIdx.x / 2u, u_step = gridDim.x / 2u;
+  // a cluster takes a tile; with K splits only one (the exchange reuses the ring)
+  const uint32_t splits = A.splits, split = cta / 2u;
+  const uint32_t total = A.row_tiles * A.token_tiles, u_begin = blockIdx.x / (2u * splits), u_step = gridDim.x / (2u * splits);
+  const uint32_t kb0 = A.stages * split / splits, kb1 = A.stages * (split + 1u) / splits;
 
   if (warp == (uint32_t)kProducerWarp) {
     // this CTA's 128 weight rows and its half of the tokens
@@ -556,11 +630,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linea
       uint32_t rt, tt;
       tile_of(A, u, rt, tt);
       const int row0 = (int)(rt * 2u * kTileRows + rank * kTileRows), tok0 = (int)(tt * BN + rank * (BN / 2u));
-      for (uint32_t kb = 0; kb < A.stages; ++kb) {
+      for (uint32_t kb = kb0; kb < kb1; ++kb) {
         if (lwait(sh, &sh.empty[slot], phase ^ 1u, a.flags)) {
           uint8_t *dst = sh.ring + slot * C::STAGE;
           if (elect_one()) {
-            const uint32_t bar = map_rank(smem_addr(&sh.full[slot]), 0u);
+            const uint32_t bar = map_rank(smem_addr(&sh.full[slot]), lead);
             if (rank == 0u) mbar_arrive_expect_tx(&sh.full[slot], 2u * C::STAGE);
             if (A.k3d) {
               tma_load_pair(dst, &A.wmap, 0, row0, (int)kb, bar);
@@ -594,7 +668,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linea
         const bool ok_acc = lwait<true>(sh, &sh.tempty[acc], aphase ^ 1u, a.flags);
         tc_fence_after();
         const uint32_t d = tmem + acc * BN;
-        for (uint32_t kb = 0; kb < A.stages; ++kb) {
+        for (uint32_t kb = kb0; kb < kb1; ++kb) {
           const bool ok = lwait(sh, &sh.full[slot], phase, a.flags) && ok_acc;
           tc_fence_after();
           if (ok) {
@@ -602,15 +676,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linea
             const uint64_t bd = ad + (C::A_BYTES >> 4);
 #pragma unroll
             for (uint32_t s = 0; s < 4; ++s)
-              mma_f16_pair_elect(d, ad + 2u * s, bd + 2u * s, idesc, (kb | s) ? 1u : 0u);
+              mma_f16_pair_elect(d, ad + 2u * s, bd + 2u * s, idesc, (kb != kb0 || s) ? 1u : 0u);
           }
-          mma_commit_pair_elect(&sh.empty[slot]);
+          mma_commit_pair_elect(&sh.empty[slot], 3u << lead);
           if (++slot == NST) {
             slot = 0;
             phase ^= 1u;
           }
         }
-        mma_commit_pair_elect(&sh.tfull[acc]);
+        mma_commit_pair_elect(&sh.tfull[acc], 3u << lead);
         pending |= 1u << acc;
         pend_parity = (pend_parity & ~(1u << acc)) | (aphase << acc);
         if (++acc == 2u) {
@@ -630,19 +704,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linea
     for (uint32_t u = u_begin; u < total; u += u_step) {
       uint32_t rt, tt;
       tile_of(A, u, rt, tt);
-      const uint32_t c = rt * 2u * kTileRows + rank * kTileRows + quarter * 32u + lane;
+      const uint32_t row = quarter * 32u + lane, c = rt * 2u * kTileRows + rank * kTileRows + row;
       const bool mine = c < a.rows;
       const float bias = mine && a.ep.bias ? load_elem(a.ep.bias, c, a.ep.bias_dtype) : 0.0f;
       // 32 tokens at a time, their residual loaded one step ahead (the first
       // while the tile's products still run)
       const uint32_t t_begin = tt * BN + col0;
-      const bool add = mine && a.ep.residual != nullptr;
+      const bool add = mine && a.ep.residual != nullptr && splits == 1u;
       uint32_t raw[32];
-      if (add && t_begin < a.width) load_residual32(a.ep, t_begin, c, min(32u, a.width - t_begin), raw);
+      if (add && t_begin < a.width) load_residual(a.ep, t_begin, c, min(32u, a.width - t_begin), raw);
       const bool ok = __all_sync(0xffffffffu, lwait(sh, &sh.tfull[acc], aphase, a.flags));
       tc_fence_after();
       const uint32_t src = tmem + ((quarter * 32u) << 16) + acc * BN + col0;
-      if (ok) {
+      if (splits > 1u) {
+        const Exchange x(sh.ring, splits, split, 2u, rank, min(BN, a.width - tt * BN));
+        __syncwarp();
+        cluster_sync_all();  // every pair's MMAs have read their last stage
+        if (ok) {
+#pragma unroll 1
+          for (uint32_t q = 0; q < BN / 2u; q += 32u) {
+            float v[32];
+            tc::tmem_ld32(src + q, v);
+            tc::tmem_wait_ld(v);
+            x.send32(v, col0 + q, row);
+          }
+        }
+        finish_share(x, a, bias, tt * BN, c, row, half);
+      } else if (ok) {
 #pragma unroll 1
         for (uint32_t q = 0; q < BN / 2u; q += 32u) {
           float v[32];
@@ -652,14 +740,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linea
           uint32_t cur[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) cur[j] = raw[j];
-          if (add && q + 32u < BN / 2u && t1 < a.width) load_residual32(a.ep, t1, c, min(32u, a.width - t1), raw);
-          if (mine && t0 < a.width) finish32(a.ep, v, bias, cur, t0, c, min(32u, a.width - t0), a.flags);
+          if (add && q + 32u < BN / 2u && t1 < a.width) load_residual(a.ep, t1, c, min(32u, a.width - t1), raw);
+          if (mine && t0 < a.width) finish(a.ep, v, bias, cur, t0, c, min(32u, a.width - t0), a.flags);
           __syncwarp();
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_remote(map_rank(smem_addr(&sh.tempty[acc]), 0u));
+      if (lane == 0) arrive_remote(map_rank(smem_addr(&sh.tempty[acc]), lead));
       if (++acc == 2u) {
         acc = 0;
         aphase ^= 1u;
@@ -667,6 +755,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_linea
     }
   }
 
+  if (A.splits > 1u && warp < (uint32_t)kEpiWarp0) {
+    // the epilogue's two cluster barriers count every thread
+    __syncwarp();
+    cluster_sync_all();
+    cluster_sync_all();
+  }
   tc_fence_before();
   __syncthreads();
   __syncwarp();
@@ -692,30 +786,72 @@ bool make_args(const LinearArgs &a, uint32_t rows, uint32_t tokens, uint32_t box
   return (uint64_t)A.row_tiles * A.token_tiles <= 0x7fffffffull / kMaxSplits;
 }
 
+// A launch of `cluster` CTAs per cluster (1: none).
+struct Launch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  Launch(uint32_t grid, uint32_t cluster, uint32_t smem, cudaStream_t stream) {
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1u ? 2 : 1;
+  }
+};
+
+// Clusters of each size that run at once.  An SM holds one CTA, and a cluster
+// stays within a GPC, so sizes that do not divide the GPCs leave SMs idle (of a
+// B200's 148: 132 CTAs in clusters of 4 or 6, 120 in clusters of 8).
+template <auto Kernel>
+uint32_t clusters_at_once(uint32_t cluster, uint32_t smem, int num_sms) {
+  static std::atomic<int> known[kMaxSplits + 1];
+  if (cluster == 1u) return (uint32_t)num_sms;
+  int n = known[cluster].load(std::memory_order_relaxed);
+  if (n == 0) {
+    Launch l(cluster, cluster, smem, nullptr);
+    if (cudaOccupancyMaxActiveClusters(&n, Kernel, &l.cfg) != cudaSuccess || n < 1) n = num_sms / (int)kMaxSplits;
+    known[cluster].store(n, std::memory_order_relaxed);
+  }
+  return (uint32_t)n;
+}
+
+// K splits of `tiles` tiles: the count with the least time over waves of
+// clusters.  A k-block takes about 512 cycles either way (a pair's products; a
+// tile's operands through L2), a wave 4000 more, with the exchange 8000.  Every
+// split keeps four k-blocks.
+template <auto Kernel>
+uint32_t best_splits(uint64_t tiles, uint32_t k_blocks, uint32_t most, uint32_t cta_per_split, uint32_t smem, int num_sms) {
+  uint32_t best = 1u;
+  uint64_t least = ~(uint64_t)0;
+  for (uint32_t s = 1u; s <= most && (s == 1u || s * 4u <= k_blocks); ++s) {
+    const uint64_t n = clusters_at_once<Kernel>(s * cta_per_split, smem, num_sms);
+    const uint64_t waves = (tiles + n - 1u) / n, cost = waves * ((uint64_t)k_blocks * 512u / s + (s > 1u ? 8000u : 4000u));
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
+
 template <int BN>
-cudaError_t launch_tile(const LinearArgs &a, uint32_t splits, int num_sms, cudaStream_t stream) {
+cudaError_t launch_tile(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   using C = TileCfg<BN>;
   Args A{};
   if (!make_args(a, kTileRows, BN, BN, C::KBS, A)) return cudaErrorInvalidValue;
   cudaError_t e = allow_smem<k_linear_tile<BN>>(C::SMEM);
   if (e != cudaSuccess) return e;
-  A.splits = splits;
-  const uint32_t tiles = A.row_tiles * A.token_tiles;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits > 1u ? tiles * splits : tiles < (uint32_t)num_sms ? tiles : (uint32_t)num_sms);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = splits;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = splits > 1u ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, k_linear_tile<BN>, A);
+  const uint32_t tiles = A.row_tiles * A.token_tiles, sms = (uint32_t)num_sms;
+  A.splits = best_splits<k_linear_tile<BN>>(tiles, A.stages * C::KBS, kMaxSplits, 1u, C::SMEM, num_sms);
+  Launch l(A.splits > 1u ? tiles * A.splits : tiles < sms ? tiles : sms, A.splits, C::SMEM, stream);
+  e = cudaLaunchKernelEx(&l.cfg, k_linear_tile<BN>, A);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -726,7 +862,10 @@ cudaError_t launch_pair(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   cudaError_t e = allow_smem<k_linear_pair>(C::SMEM);
   if (e != cudaSuccess) return e;
   const uint32_t tiles = A.row_tiles * A.token_tiles, pairs = (uint32_t)num_sms / 2u;
-  return launch_kernel(k_linear_pair, dim3(2u * (tiles < pairs ? tiles : pairs)), dim3(kThreads), C::SMEM, stream, A);
+  A.splits = best_splits<k_linear_pair>(tiles, A.stages, kMaxSplits / 2u, 2u, C::SMEM, num_sms);
+  Launch l(2u * (A.splits > 1u ? tiles * A.splits : tiles < pairs ? tiles : pairs), 2u * A.splits, C::SMEM, stream);
+  e = cudaLaunchKernelEx(&l.cfg, k_linear_pair, A);
+  return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 // ------------------------------------------------------------- row conversion
@@ -757,24 +896,10 @@ cudaError_t launch_linear(const LinearArgs &a, int num_sms, cudaStream_t stream)
   if (a.rows == 0 || a.cols == 0 || (a.dtype != PW_DTYPE_BF16 && a.dtype != PW_DTYPE_F16)) return cudaErrorInvalidValue;
   if (a.width == 0) return cudaSuccess;
   if (a.width <= 16u) return launch_linear_narrow(a, num_sms, stream);
-  // Tiles of one CTA: as many K splits as fill the SMs, each of two stages or more.
-  const uint64_t sms = (uint64_t)num_sms;
-  const uint32_t bn = a.width <= 32u ? 32u : a.width <= 64u ? 64u : 128u;
-  const uint64_t tiles = (uint64_t)((a.rows + lin::kTileRows - 1u) / lin::kTileRows) * ((a.width + bn - 1u) / bn);
-  const uint32_t stages = (a.cols + 2u * lin::kBlockK - 1u) / (2u * lin::kBlockK);
-  uint64_t splits = sms / (tiles ? tiles : 1u);
-  splits = splits > stages / 2u ? stages / 2u : splits;
-  splits = splits > lin::kMaxSplits ? lin::kMaxSplits : splits < 1u ? 1u : splits;
-  // Pairs do two such tiles' work per CTA and tile, at about 1.5 times the rate
-  // (shared memory feeds the 128 x 128 tile's products at 2/3 of the tensor
-  // rate), but cannot split K.
-  const uint64_t pair_tiles = (uint64_t)((a.rows + 255u) / 256u) * ((a.width + 255u) / 256u);
-  const double pair_cost = (double)((pair_tiles + sms / 2u - 1u) / (sms / 2u)) * 2.0;
-  const double tile_cost = (double)((tiles * splits + sms - 1u) / sms) / (double)splits * 1.5;
-  if (a.ep.y_dtype != PW_DTYPE_F32 && a.width > 128u && pair_cost <= tile_cost) return lin::launch_pair(a, num_sms, stream);
-  if (bn == 32u) return lin::launch_tile<32>(a, (uint32_t)splits, num_sms, stream);
-  if (bn == 64u) return lin::launch_tile<64>(a, (uint32_t)splits, num_sms, stream);
-  return lin::launch_tile<128>(a, (uint32_t)splits, num_sms, stream);
+  if (a.ep.y_dtype != PW_DTYPE_F32 && a.width > 128u) return lin::launch_pair(a, num_sms, stream);
+  if (a.width <= 32u) return lin::launch_tile<32>(a, num_sms, stream);
+  if (a.width <= 64u) return lin::launch_tile<64>(a, num_sms, stream);
+  return lin::launch_tile<128>(a, num_sms, stream);
 }
 
 }  // namespace pw

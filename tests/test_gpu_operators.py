@@ -238,7 +238,8 @@ def test_linear_sums_are_exact_on_small_integers(rt, width, rows, cols, dtype):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("width,rows,cols", [(1500, 2600, 64), (700, 4100, 72), (1500, 3001, 1003), (1030, 5130, 456),
-                                             (2048, 4096, 1856), (129, 9500, 128)])
+                                             (2048, 4096, 1856), (129, 9500, 128), (200, 1000, 1003), (300, 600, 1992),
+                                             (131, 256, 1536), (517, 4096, 520), (140, 200, 60)])
 def test_wide_linear_sums_are_exact_on_small_integers(rt, width, rows, cols, dtype):
     # sums of products of -1, 0 and 1 stay below 2048: exact in f16 too
     t = TYPES[dtype]
