@@ -343,9 +343,10 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
 /* pw_fp8_linear on activations that are already quantized (pw_quantize_fp8,
  * pw_add_rms_norm), with the epilogue of pw_linear: codes u8 [width, cols] and
  * scales f32 [width, cols / 128], contiguous, y [width, rows] of any dtype.
- * The sums are those of pw_fp8_linear (the same kernels), so y of dtype F32
- * without an epilogue equals its PW_OUTPUT_F32 output bit for bit.  Shapes as
- * in pw_fp8_linear; codes start at a 16-byte boundary. */
+ * Each 128-column block's product is promoted by its two scales in f32, as in
+ * pw_fp8_linear; the blocks may be added in another order (a different f32
+ * rounding, nothing else).  Shapes as in pw_fp8_linear; codes start at a 16-byte
+ * boundary. */
 int pw_fp8_linear_codes(pw_runtime *rt, const pw_fp8_tensor *w, uint32_t layout, const uint8_t *codes,
                         const float *scales, uint32_t width, const pw_epilogue *ep, const pw_rows *y, uint32_t mem,
                         pw_stats *stats);

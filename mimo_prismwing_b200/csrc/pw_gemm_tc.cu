@@ -39,7 +39,6 @@
 #include <cuda_runtime.h>
 
 #include "pw_device.cuh"
-#include "pw_epilogue.cuh"
 #include "pw_internal.h"
 #include "pw_tc.cuh"
 
@@ -156,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm_tc(const __grid_constant__
   const uint32_t kblocks = a.K / 128u;
   const uint32_t kcs = (kblocks + 1u) / 2u;          // stages per matrix per tile
   const uint32_t per_tile = kcs * (uint32_t)MATS;   // stages per tile; fused: all gate, then all up
-  const bool qkv = (KIND == 0 || KIND == 4) && a.layout != PW_LAYOUT_PLAIN;
+  const bool qkv = KIND == 0 && a.layout != PW_LAYOUT_PLAIN;
 
   if (warp == kProducerWarp) {
     // converged like the MMA warp: every lane waits, one elected lane issues
@@ -422,34 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm_tc(const __grid_constant__
         }
         __syncwarp();  // the staging rows are rewritten by the next piece
       };
-      if (KIND == 4) {
-        // The linear layers' epilogue.  The f32 sums pass through the staging
-        // rows 16 columns at a time; the thread that stores four columns of a
-        // row applies bias, activation and residual.  The loop over the rows
-        // stays rolled: unrolled over all 64 values the activations' code
-        // (five formulas each) ran out of the instruction cache and the
-        // epilogue took three times as long as the tile's products.
-        const EpilogueArgs &ep = a.ep;
-        bool ok = true;
-#pragma unroll
-        for (uint32_t h = 0; h < 4; ++h) {
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i)
-            *reinterpret_cast<float4 *>(stg + lane * 64u + ((i ^ ((lane >> 1) & 3u)) << 4)) =
-                make_float4(acc[8 * h + 2 * i].x, acc[8 * h + 2 * i].y, acc[8 * h + 2 * i + 1].x,
-                            acc[8 * h + 2 * i + 1].y);
-          __syncwarp();
-          const uint32_t c = lane % 4u, col = row0 + col0 + h * 16u + c * 4u;
-          const float4 bias = bias4(ep, col);
-#pragma unroll 1
-          for (uint32_t r = lane / 4u; r < rows_here; r += 8u) {
-            const float4 v = *reinterpret_cast<const float4 *>(stg + r * 64u + ((c ^ ((r >> 1) & 3u)) << 4));
-            ok = finish4(ep, v, bias, p0 + r, col) && ok;
-          }
-          __syncwarp();
-        }
-        if (!ok) raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
-      } else if (KIND != 2) {
+      if (KIND != 2) {
         // bf16 rounding by the conversion instruction; an output is non-finite
         // when its f32 sum is, or when rounding carries it past the largest bf16
         const bool rb = a.round_bf16 != 0u;
@@ -571,13 +543,12 @@ int gemm_tc_tokens(int) { return tc::kTN; }
 cudaError_t launch_gemm_tc(int kind, const GemmArgs &a, int grid, cudaStream_t stream) {
   const GemvArgs &g = a.g;
   if (g.K == 0 || g.K % 128u || g.K > 4096u || g.rows % tc::kTileRows || grid <= 0 ||
-      (g.layout != PW_LAYOUT_PLAIN && kind != 0 && kind != 4))
+      (g.layout != PW_LAYOUT_PLAIN && kind != 0))
     return cudaErrorInvalidValue;
   switch (kind) {
     case 0: return tc::launch_one<0>(a, grid, stream);
     case 2: return tc::launch_one<2>(a, grid, stream);
     case 3: return tc::launch_one<3>(a, grid, stream);
-    case 4: return tc::launch_one<4>(a, grid, stream);
     default: return cudaErrorInvalidValue;
   }
 }

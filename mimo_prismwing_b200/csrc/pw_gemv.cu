@@ -122,7 +122,6 @@ cudaError_t launch_gemv(int kind, const GemvArgs &a, int grid, cudaStream_t stre
     case 0:
     case 2:
     case 3:
-    case 4:
       // Plain row-major weights, whole-K units: the tcgen05 GEMV (decode
       // layer at width 8: 282 -> 264 us).  Fused-QKV shard maps (64-row
       // boxes) and split-K launches (a lone expert: 1/8-tile units, where the

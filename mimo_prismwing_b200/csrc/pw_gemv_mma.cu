@@ -40,7 +40,6 @@
 #include <cuda_runtime.h>
 
 #include "pw_device.cuh"
-#include "pw_epilogue.cuh"
 #include "pw_internal.h"
 
 namespace pw {
@@ -477,15 +476,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemv_mma(const GemvArgs a, cons
     for (int i = 0; i < 4; ++i) {
       const uint32_t t = tig * 2u + (i & 1u);
       float out = 0.0f;
-      if (KIND == 4) {
-        if (t < grp.count) {
-          const uint64_t tok = grp.tok_begin + t;
-          const uint32_t c = row0 + warp * 16u + gid + (i >= 2 ? 8u : 0u);
-          if (!store_elem(a.ep.y, tok * a.ep.y_stride + c, a.ep.y_dtype, epilogue_value(a.ep, acc[0][i], tok, c)))
-            raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
-        }
-        continue;
-      }
       if (t < grp.count) {
         if (FUSED) {
           out = staged_swiglu(acc[0][i], acc[MATS - 1][i]);
@@ -570,7 +560,6 @@ cudaError_t launch_gemv_mma(int kind, const GemvArgs &a, int grid, cudaStream_t 
     case 0: return mma::launch_one<0>(a, grid, stream);
     case 2: return mma::launch_one<2>(a, grid, stream);
     case 3: return mma::launch_one<3>(a, grid, stream);
-    case 4: return mma::launch_one<4>(a, grid, stream);
     default: return cudaErrorInvalidValue;
   }
 }

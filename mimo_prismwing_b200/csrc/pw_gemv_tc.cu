@@ -43,7 +43,6 @@
 #include <cuda_runtime.h>
 
 #include "pw_device.cuh"
-#include "pw_epilogue.cuh"
 #include "pw_internal.h"
 #include "pw_tc.cuh"
 
@@ -153,8 +152,7 @@ __device__ __forceinline__ void tree_add(float (&acc)[MATS][4], const float (&le
 }
 
 // KIND 0: one projection (w0); 2: fused gate (w0) / up (w1) + staged SwiGLU +
-// the hidden's dynamic FP8 quantization; 3: one projection of w1 (up); 4: kind
-// 0 with the linear layers' epilogue.
+// the hidden's dynamic FP8 quantization; 3: one projection of w1 (up).
 template <int KIND>
 __global__ void __launch_bounds__(kThreads, 1) k_gemv_tc(const GemvArgs a, const uint32_t nst) {
   constexpr bool FUSED = KIND == 2;
@@ -482,15 +480,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemv_tc(const GemvArgs a, const
       for (int i = 0; i < 4; ++i) {
         const uint32_t t = t0 + (uint32_t)i;
         float out = 0.0f;
-        if (KIND == 4) {
-          if (t < grp.count) {
-            const uint64_t tok = grp.tok_begin + t;
-            const uint32_t c = row0 + r_loc;
-            if (!store_elem(a.ep.y, tok * a.ep.y_stride + c, a.ep.y_dtype, epilogue_value(a.ep, acc[0][i], tok, c)))
-              raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
-          }
-          continue;
-        }
         if (t < grp.count) {
           if (FUSED) {
             out = staged_swiglu(acc[0][i], acc[MATS - 1][i]);
@@ -573,7 +562,6 @@ cudaError_t launch_gemv_tc(int kind, const GemvArgs &a, int grid, cudaStream_t s
     case 0: return gtc::launch_one<0>(a, grid, stream);
     case 2: return gtc::launch_one<2>(a, grid, stream);
     case 3: return gtc::launch_one<3>(a, grid, stream);
-    case 4: return gtc::launch_one<4>(a, grid, stream);
     default: return cudaErrorInvalidValue;
   }
 }

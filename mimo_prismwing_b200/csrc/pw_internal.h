@@ -122,7 +122,6 @@ struct GemvArgs {
   const GemvGroup *l2_next;      // optional: the next kernel's groups (same count); CTAs with
   uint32_t l2_rows, l2_cols;     //   no unit of their own prefetch those groups' w0 [rows, cols]
                                  //   into L2 while the others stream
-  EpilogueArgs ep;               // kind 4: bias, activation, residual and the output rows
 };
 
 // Wide-width grouped GEMM (tcgen05): the GEMV arguments plus TMA maps of the
@@ -149,8 +148,7 @@ cudaError_t launch_quantize(const float *x, uint32_t rows, uint32_t cols, uint8_
                             uint32_t *zero = nullptr, uint32_t n_zero = 0);
 // kind: 0 = block-scaled (quantized x) over each group's w0/s0, 1 = readable
 // (f32 x), 2 = fused gate/up SwiGLU over w0/s0 and w1/s1, 3 = block-scaled
-// over w1/s1 (the unfused up projection), 4 = kind 0 with the epilogue `ep`
-// (pw_epilogue.cuh) instead of `out` / `round_bf16`
+// over w1/s1 (the unfused up projection)
 cudaError_t launch_gemv(int kind, const GemvArgs &args, int grid, cudaStream_t stream);
 int gemv_max_ctas(int num_sms);
 cudaError_t launch_gemv_mma(int kind, const GemvArgs &args, int grid, cudaStream_t stream);
@@ -282,6 +280,20 @@ cudaError_t launch_convert_rows(const void *x, uint64_t x_stride, uint32_t x_dty
 // view {cols, rows, 1} in boxes {64, box_rows, 1}, zero past the last column.
 bool encode_rows16_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride,
                        uint32_t dtype, uint32_t box_rows, uint32_t k_blocks);
+
+// Block-scaled FP8 linear layer on codes [width, K] with scales [width, K / 128]:
+// weight [rows, K] e4m3 in `layout`, ws its scale grid (K / 128 columns).
+struct Fp8CodesArgs {
+  const uint8_t *w;
+  const float *ws;
+  const uint8_t *codes;  // 16-byte aligned
+  const float *scales;
+  uint32_t rows, K, layout, width;
+  EpilogueArgs ep;
+  uint32_t *flags;
+};
+cudaError_t launch_fp8_narrow(const Fp8CodesArgs &a, cudaStream_t stream);  // up to 16 tokens
+cudaError_t launch_fp8_gemm(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream);
 
 // Expert-parallel window of one rank (byte offsets from its base): flags
 // written by peers (ready for an epoch, data sent, rows returned), the

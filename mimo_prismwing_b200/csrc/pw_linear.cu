@@ -31,6 +31,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "pw_cluster.cuh"
 #include "pw_device.cuh"
 #include "pw_epilogue.cuh"
 #include "pw_internal.h"
@@ -39,6 +40,7 @@
 namespace pw {
 namespace lin {
 
+using namespace clu;
 using tc::elect_one;
 using tc::smem_desc_sw128;
 using tc::tc_fence_after;
@@ -49,11 +51,9 @@ constexpr int kMmaWarp = 1;
 constexpr int kEpiWarp0 = 2;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
-constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kBlockK = 64;        // columns of a k-block: one 128-byte line
 constexpr uint32_t kSmemLimit = 227u * 1024u;
 constexpr uint32_t kTokenGroup = 8;     // token tiles that neighbouring CTAs share weights over
-constexpr uint32_t kMaxSplits = 8;
 
 template <int BN>
 struct TileCfg {
@@ -121,96 +121,12 @@ __device__ __forceinline__ void mma_f16_pair_elect(uint32_t d, uint64_t a, uint6
       "l"(a), "l"(b), "r"(idesc), "r"(accum)
       : "memory");
 }
-// Arrives on the barrier at this offset in both CTAs once the MMAs so far are complete.
-__device__ __forceinline__ void mma_commit_pair_elect(uint64_t *bar, uint32_t pair_mask) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
-          smem_addr(bar)),
-      "h"((uint16_t)pair_mask)
-      : "memory");
-}
-// A tile load into this CTA's shared memory that completes on the pair's
-// leading CTA's barrier (a shared::cluster address).
-__device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-      "%4}], [%5];" ::"r"(smem_addr(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
-}
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-// The address of this CTA's shared-memory location in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void arrive_remote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void store_remote4(uint32_t addr, float x, float y, float z, float w) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
-
 struct Shared {
   uint8_t *ring;
   uint64_t *full, *empty, *tfull, *tempty;
   uint32_t *tmem_base;
   volatile int *abort;
 };
-
-// Bounded wait (1 s) that sleeps in hardware between looks: ten warps polling in
-// a loop took a fifth of the ALU's issue slots and, under the power cap, clock
-// from the tensor pipe.  PAIR: the pair's other CTA arrives on the barrier too.
-template <bool PAIR>
-__device__ __forceinline__ bool try_wait_sleep(uint64_t *bar, uint32_t parity) {
-  constexpr uint32_t kSleepNs = 100000;  // at most; the phase's completion wakes the thread
-  uint32_t done;
-  if (PAIR)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(kSleepNs)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(kSleepNs)
-        : "memory");
-  return done != 0u;
-}
-
-template <bool PAIR = false>
-__device__ __forceinline__ bool lwait(const Shared &sh, uint64_t *bar, uint32_t parity, uint32_t *flags) {
-  if (*sh.abort) return false;
-  if (try_wait_sleep<PAIR>(bar, parity)) return true;
-  const uint64_t start = global_timer_ns();
-  do {
-    if (try_wait_sleep<PAIR>(bar, parity)) return true;
-  } while (global_timer_ns() - start <= kWaitLimitNs);
-  *sh.abort = 1;
-  raise_flag(flags, PW_FLAG_WAIT_TIMEOUT);
-  return false;
-}
 
 // Tile u: neighbouring tiles share their token tiles within a group of
 // kTokenGroup, so that the tiles in flight reuse both operands in L2.
@@ -277,56 +193,6 @@ __device__ __forceinline__ void finish(const EpilogueArgs &e, float (&v)[N], flo
   else store_rows(v, static_cast<__half *>(e.y) + at, e.y_stride, n);
 }
 
-// Joining K splits.  Split k of a tile finishes tokens [k share, (k + 1) share) of
-// the tile's `tokens`; share is a multiple of 8, so that a quad of tokens has one
-// owner and each half of the epilogue warps whole quads.  The sums travel as
-// [source split][quad of the share][128 rows][4 tokens] f32.
-struct Exchange {
-  uint32_t ring;    // this CTA's ring
-  uint32_t splits, split, step, base;  // split k is the cluster's CTA base + step k
-  uint32_t tokens, share;
-  __device__ __forceinline__ Exchange(uint8_t *r, uint32_t n_splits, uint32_t k, uint32_t cta_step, uint32_t cta_base,
-                                      uint32_t n_tokens)
-      : ring(smem_addr(r)), splits(n_splits), split(k), step(cta_step), base(cta_base), tokens(n_tokens) {
-    share = ((n_tokens + n_splits - 1u) / n_splits + 7u) & ~7u;
-  }
-  __device__ __forceinline__ uint32_t slot(uint32_t from, uint32_t token_of_share, uint32_t row) const {
-    return ((from * (share / 4u) + token_of_share / 4u) * kTileRows + row) * 16u;
-  }
-  // this row's sums of tile tokens t0 .. t0 + 31 (t0 % 32 == 0) to their owners
-  __device__ __forceinline__ void send32(const float (&v)[32], uint32_t t0, uint32_t row) const {
-    uint32_t to = t0 / share, at = t0 % share;
-    uint32_t dst = to < splits ? map_rank(ring + slot(split, 0u, row), base + step * to) : 0u;
-#pragma unroll
-    for (uint32_t q = 0; q < 8; ++q) {
-      if (t0 + 4u * q < tokens) store_remote4(dst + slot(0u, at, 0u), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-      at += 4u;
-      if (at == share && to + 1u < splits) {
-        at = 0u;
-        ++to;
-        dst = map_rank(ring + slot(split, 0u, row), base + step * to);
-      }
-    }
-  }
-  // this row's joined sums of tokens b .. b + 7 of this CTA's share
-  __device__ __forceinline__ void receive8(float (&v)[8], uint32_t b, uint32_t row) const {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    for (uint32_t s = 0; s < splits; ++s)
-#pragma unroll
-      for (uint32_t q = 0; q < 2; ++q) {
-        float x, y, z, w;
-        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(x), "=f"(y), "=f"(z), "=f"(w)
-                     : "r"(ring + slot(s, b + 4u * q, row)));
-        v[4 * q] += x;
-        v[4 * q + 1] += y;
-        v[4 * q + 2] += z;
-        v[4 * q + 3] += w;
-      }
-  }
-};
-
 // The rest of a split tile's epilogue, from the CTA's own sums sent: joins and
 // finishes this thread's row (output column c) for its half of the share, 8
 // tokens at a time (each CTA runs this once: a short loop, because code that is
@@ -336,7 +202,7 @@ __device__ __forceinline__ void finish_share(const Exchange &x, const LinearArgs
   const bool mine = c < a.rows;
   const uint32_t first = x.split * x.share, mid = x.share / 2u & ~7u;
   // tokens [begin, end) of the share
-  const uint32_t in_tile = first < x.tokens ? min(x.share, x.tokens - first) : 0u;
+  const uint32_t in_tile = first < x.cols ? min(x.share, x.cols - first) : 0u;
   const uint32_t begin = half ? mid : 0u, end = half ? in_tile : min(mid, in_tile);
   uint32_t raw[8];
   const bool add = mine && a.ep.residual != nullptr;
@@ -415,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tile(const __grid_consta
       tile_of(A, u, rt, tt);
       const int row0 = (int)(rt * kTileRows), tok0 = (int)(tt * BN);
       for (uint32_t st = st0; st < st1; ++st) {
-        if (lwait(sh, &sh.empty[slot], phase ^ 1u, a.flags)) {
+        if (bounded_wait(sh.abort, &sh.empty[slot], phase ^ 1u, a.flags)) {
           uint8_t *dst = sh.ring + slot * C::STAGE;
           const int kb = (int)(st * C::KBS);
           if (elect_one()) {
@@ -455,10 +321,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tile(const __grid_consta
       for (uint32_t st = st0; st < st1; ++st) {
         const uint32_t in_seg = (st - st0) % C::SEG;
         if (in_seg == 0u) {
-          ok_acc = lwait(sh, &sh.tempty[acc], aphase ^ 1u, a.flags);
+          ok_acc = bounded_wait(sh.abort, &sh.tempty[acc], aphase ^ 1u, a.flags);
           tc_fence_after();
         }
-        const bool ok = lwait(sh, &sh.full[slot], phase, a.flags) && ok_acc;
+        const bool ok = bounded_wait(sh.abort, &sh.full[slot], phase, a.flags) && ok_acc;
         tc_fence_after();
         if (ok) {
           const uint32_t d = tmem + acc * (uint32_t)BN;
@@ -512,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tile(const __grid_consta
 #pragma unroll
         for (int j = 0; j < 32; ++j) sum[q][j] = 0.0f;
       for (uint32_t st = st0; st < st1; st += C::SEG) {
-        const bool ok = __all_sync(0xffffffffu, lwait(sh, &sh.tfull[acc], aphase, a.flags));
+        const bool ok = __all_sync(0xffffffffu, bounded_wait(sh.abort, &sh.tfull[acc], aphase, a.flags));
         tc_fence_after();
         if (ok && active) {
           const uint32_t src = tmem + ((quarter * 32u) << 16) + acc * (uint32_t)BN + col0;
@@ -631,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_pair(const __grid_consta
       tile_of(A, u, rt, tt);
       const int row0 = (int)(rt * 2u * kTileRows + rank * kTileRows), tok0 = (int)(tt * BN + rank * (BN / 2u));
       for (uint32_t kb = kb0; kb < kb1; ++kb) {
-        if (lwait(sh, &sh.empty[slot], phase ^ 1u, a.flags)) {
+        if (bounded_wait(sh.abort, &sh.empty[slot], phase ^ 1u, a.flags)) {
           uint8_t *dst = sh.ring + slot * C::STAGE;
           if (elect_one()) {
             const uint32_t bar = map_rank(smem_addr(&sh.full[slot]), lead);
@@ -665,11 +531,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_pair(const __grid_consta
       const uint64_t ring_desc = smem_desc_sw128(smem_addr(sh.ring));
       uint32_t slot = 0, phase = 0, acc = 0, aphase = 0, pending = 0, pend_parity = 0;
       for (uint32_t u = u_begin; u < total; u += u_step) {
-        const bool ok_acc = lwait<true>(sh, &sh.tempty[acc], aphase ^ 1u, a.flags);
+        const bool ok_acc = bounded_wait<true>(sh.abort, &sh.tempty[acc], aphase ^ 1u, a.flags);
         tc_fence_after();
         const uint32_t d = tmem + acc * BN;
         for (uint32_t kb = kb0; kb < kb1; ++kb) {
-          const bool ok = lwait(sh, &sh.full[slot], phase, a.flags) && ok_acc;
+          const bool ok = bounded_wait(sh.abort, &sh.full[slot], phase, a.flags) && ok_acc;
           tc_fence_after();
           if (ok) {
             const uint64_t ad = ring_desc + ((slot * C::STAGE) >> 4);
@@ -713,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_pair(const __grid_consta
       const bool add = mine && a.ep.residual != nullptr && splits == 1u;
       uint32_t raw[32];
       if (add && t_begin < a.width) load_residual(a.ep, t_begin, c, min(32u, a.width - t_begin), raw);
-      const bool ok = __all_sync(0xffffffffu, lwait(sh, &sh.tfull[acc], aphase, a.flags));
+      const bool ok = __all_sync(0xffffffffu, bounded_wait(sh.abort, &sh.tfull[acc], aphase, a.flags));
       tc_fence_after();
       const uint32_t src = tmem + ((quarter * 32u) << 16) + acc * BN + col0;
       if (splits > 1u) {
@@ -786,61 +652,6 @@ bool make_args(const LinearArgs &a, uint32_t rows, uint32_t tokens, uint32_t box
   return (uint64_t)A.row_tiles * A.token_tiles <= 0x7fffffffull / kMaxSplits;
 }
 
-// A launch of `cluster` CTAs per cluster (1: none).
-struct Launch {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[2];
-  Launch(uint32_t grid, uint32_t cluster, uint32_t smem, cudaStream_t stream) {
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1u ? 2 : 1;
-  }
-};
-
-// Clusters of each size that run at once.  An SM holds one CTA, and a cluster
-// stays within a GPC, so sizes that do not divide the GPCs leave SMs idle (of a
-// B200's 148: 132 CTAs in clusters of 4 or 6, 120 in clusters of 8).
-template <auto Kernel>
-uint32_t clusters_at_once(uint32_t cluster, uint32_t smem, int num_sms) {
-  static std::atomic<int> known[kMaxSplits + 1];
-  if (cluster == 1u) return (uint32_t)num_sms;
-  int n = known[cluster].load(std::memory_order_relaxed);
-  if (n == 0) {
-    Launch l(cluster, cluster, smem, nullptr);
-    if (cudaOccupancyMaxActiveClusters(&n, Kernel, &l.cfg) != cudaSuccess || n < 1) n = num_sms / (int)kMaxSplits;
-    known[cluster].store(n, std::memory_order_relaxed);
-  }
-  return (uint32_t)n;
-}
-
-// K splits of `tiles` tiles: the count with the least time over waves of
-// clusters.  A k-block takes about 512 cycles either way (a pair's products; a
-// tile's operands through L2), a wave 4000 more, with the exchange 8000.  Every
-// split keeps four k-blocks.
-template <auto Kernel>
-uint32_t best_splits(uint64_t tiles, uint32_t k_blocks, uint32_t most, uint32_t cta_per_split, uint32_t smem, int num_sms) {
-  uint32_t best = 1u;
-  uint64_t least = ~(uint64_t)0;
-  for (uint32_t s = 1u; s <= most && (s == 1u || s * 4u <= k_blocks); ++s) {
-    const uint64_t n = clusters_at_once<Kernel>(s * cta_per_split, smem, num_sms);
-    const uint64_t waves = (tiles + n - 1u) / n, cost = waves * ((uint64_t)k_blocks * 512u / s + (s > 1u ? 8000u : 4000u));
-    if (cost < least) {
-      least = cost;
-      best = s;
-    }
-  }
-  return best;
-}
-
 template <int BN>
 cudaError_t launch_tile(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   using C = TileCfg<BN>;
@@ -849,8 +660,8 @@ cudaError_t launch_tile(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   cudaError_t e = allow_smem<k_linear_tile<BN>>(C::SMEM);
   if (e != cudaSuccess) return e;
   const uint32_t tiles = A.row_tiles * A.token_tiles, sms = (uint32_t)num_sms;
-  A.splits = best_splits<k_linear_tile<BN>>(tiles, A.stages * C::KBS, kMaxSplits, 1u, C::SMEM, num_sms);
-  Launch l(A.splits > 1u ? tiles * A.splits : tiles < sms ? tiles : sms, A.splits, C::SMEM, stream);
+  A.splits = best_splits<k_linear_tile<BN>>(tiles, A.stages * C::KBS, kMaxSplits, 1u, kThreads, C::SMEM, num_sms);
+  Launch l(A.splits > 1u ? tiles * A.splits : tiles < sms ? tiles : sms, kThreads, A.splits, C::SMEM, stream);
   e = cudaLaunchKernelEx(&l.cfg, k_linear_tile<BN>, A);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -862,8 +673,8 @@ cudaError_t launch_pair(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   cudaError_t e = allow_smem<k_linear_pair>(C::SMEM);
   if (e != cudaSuccess) return e;
   const uint32_t tiles = A.row_tiles * A.token_tiles, pairs = (uint32_t)num_sms / 2u;
-  A.splits = best_splits<k_linear_pair>(tiles, A.stages, kMaxSplits / 2u, 2u, C::SMEM, num_sms);
-  Launch l(2u * (A.splits > 1u ? tiles * A.splits : tiles < pairs ? tiles : pairs), 2u * A.splits, C::SMEM, stream);
+  A.splits = best_splits<k_linear_pair>(tiles, A.stages, kMaxSplits / 2u, 2u, kThreads, C::SMEM, num_sms);
+  Launch l(2u * (A.splits > 1u ? tiles * A.splits : tiles < pairs ? tiles : pairs), kThreads, 2u * A.splits, C::SMEM, stream);
   e = cudaLaunchKernelEx(&l.cfg, k_linear_pair, A);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -895,7 +706,12 @@ cudaError_t launch_convert_rows(const void *x, uint64_t x_stride, uint32_t x_dty
 cudaError_t launch_linear(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   if (a.rows == 0 || a.cols == 0 || (a.dtype != PW_DTYPE_BF16 && a.dtype != PW_DTYPE_F16)) return cudaErrorInvalidValue;
   if (a.width == 0) return cudaSuccess;
-  if (a.width <= 16u) return launch_linear_narrow(a, num_sms, stream);
+  // One token tile of the narrow kernel streams at HBM rate; its second tile
+  // costs registers, and with rows enough for every SM the tile kernel's ring is
+  // faster (16 tokens, 4096 columns: 512 rows 3.9 against 5.9 us, 4096 rows 8.8 against 8.6 us,
+  // 16384 rows 30.0 against 25.1 us).
+  if (a.width <= 8u || (a.width <= 16u && a.rows <= 16u * (uint32_t)num_sms))
+    return launch_linear_narrow(a, num_sms, stream);
   if (a.ep.y_dtype != PW_DTYPE_F32 && a.width > 128u) return lin::launch_pair(a, num_sms, stream);
   if (a.width <= 32u) return lin::launch_tile<32>(a, num_sms, stream);
   if (a.width <= 64u) return lin::launch_tile<64>(a, num_sms, stream);

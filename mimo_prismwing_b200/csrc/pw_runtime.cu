@@ -1192,17 +1192,8 @@ int pw_fp8_linear_codes(pw_runtime *rt, const pw_fp8_tensor *w, uint32_t layout,
     return fail(rt, PW_ERR_ARGUMENT, "y overlaps the activations");
   DeviceScope dev;
   CK(dev.enter(rt->device));
-  // Device-resident map and groups of each piece of the batch (a piece's
-  // records fill one descriptor slot), built on the first call of a shape.
-  constexpr uint32_t kPiece = 6144;
-  const bool wide = width >= kWideProjection;
-  const uint32_t chunk = wide ? (uint32_t)gemm_tc_tokens(4) : 8u;
-  const uint32_t box_rows = wide && layout != PW_LAYOUT_PLAIN ? 64u : map_box_rows(layout);
-  const uint32_t box_kb = wide && layout != PW_LAYOUT_PLAIN ? 1u : 0u;
   Call call{rt, mem, stats, 0};
   if ((s = call.begin()) != PW_OK) return s;
-  const bool chain = !wide && !rt->profiling;
-  PdlScope pdl(chain);
   Arena ar;
   for (int pass = 0; pass < 2; ++pass) {
     if (pass == 1) {
@@ -1225,34 +1216,12 @@ int pw_fp8_linear_codes(pw_runtime *rt, const pw_fp8_tensor *w, uint32_t layout,
       if ((s = call.stage_in(const_cast<float *>(dsc), scales, nx / 128u * 4u)) != PW_OK) return s;
       if (rr.data) CK(copy_rows(dr, rr, width, N, cudaMemcpyHostToDevice, rt->stream));
     }
-    for (uint32_t t0 = 0; t0 < width; t0 += kPiece) {
-      const uint32_t n = width - t0 < kPiece ? width - t0 : kPiece;
-      Descs D;
-      bool cached = false;
-      if ((s = get_descs(rt, 2u, n, chunk, *w, nullptr, nullptr, box_rows, box_kb, D, cached)) != PW_OK) return s;
-      if (!cached) return fail(rt, PW_ERR_UNSUPPORTED, "descriptor slot too small");
-      GemvArgs a = gemv_args(rt, D.gu, D.n_gu, N, K, layout);
-      a.x_codes = dc + (size_t)t0 * K;
-      a.x_scales = dsc + (size_t)t0 * (K / 128u);
-      a.early_weights = chain ? 1u : 0u;
-      a.ep = e;
-      pw_rows pr = dr, py = dy;
-      if (pr.data) pr.data = static_cast<uint8_t *>(pr.data) + t0 * pr.stride * elem_size(pr.dtype);
-      py.data = static_cast<uint8_t *>(py.data) + t0 * py.stride * elem_size(py.dtype);
-      set_rows(a.ep, pr, py);
+    Fp8CodesArgs f{w->weight, w->scale, dc, dsc, N, K, layout, width, e, rt->d_flags};
+    set_rows(f.ep, dr, dy);
+    {
       ProfScope ps(rt, P_PROJ, 1);
-      const uint64_t tiles = (uint64_t)D.n_gu * (N / 128u);
-      int grid = grid_for(rt, tiles);
-      if (wide) {
-        GemmArgs A{};
-        A.g = a;
-        if (!encode_act_maps(A.xmap, a.x_codes, n, K))
-          return fail(rt, PW_ERR_CUDA, "cuTensorMapEncodeTiled failed for the activations");
-        CK(launch_gemm_tc(4, A, grid, rt->stream));
-      } else {
-        if ((s = gemv_launch_setup(rt, a, tiles, 1, grid)) != PW_OK) return s;
-        CK(launch_gemv(4, a, grid, rt->stream));
-      }
+      PdlScope pdl(!rt->profiling);
+      CK(width <= 16u ? launch_fp8_narrow(f, rt->stream) : launch_fp8_gemm(f, rt->num_sms, rt->stream));
     }
     if (host) CK(copy_rows(yr, dy, width, N, cudaMemcpyDeviceToHost, rt->stream));
   }

@@ -348,21 +348,40 @@ def fp8_case(width, rows, cols, seed):
 
 
 @pytest.mark.parametrize("layout", [0, 1, 2])
-@pytest.mark.parametrize("width", [1, 3, 8, 9, 31, 32, 100, 129, 300])
-def test_fp8_codes_equal_fp8_linear(rt, width, layout):
+@pytest.mark.parametrize("width", [1, 3, 8, 9, 16, 17, 31, 32, 100, 129, 300, 1500])
+def test_fp8_codes_match_fp8_linear(rt, width, layout):
+    # two f32 evaluations of the same sum: each within linear_slack of it.  sum |x w| comes from the same
+    # projection of the magnitudes.
     from mimo_prismwing_b200.runtime import WideProjectionBinding
-    rows, scale_rows = [(512, 4), (13568, 108), (14848, 116)][layout]
+    rows, scale_rows = [(640, 5), (13568, 108), (14848, 116)][layout]
     cols = 1024 if layout == 0 else 4096
     x = randn((width, cols), 40)
     w = torch.randint(0, 256, (rows, cols), generator=gen(41), device="cuda", dtype=torch.uint8)
     w[(w & 0x7f) == 0x7f] = 0x30
     b = WideProjectionBinding(w, randn((scale_rows, cols // 128), 42).abs() * 1e-3)
     codes, scales = rt.quantize(x)
-    ref = rt.execute_fp8_linear(x, b, layout=layout, f32_output=True).output
-    assert torch.equal(rt.fp8_linear_codes(codes, scales, b, layout=layout).output, ref)
-    rounded = rt.execute_fp8_linear(x, b, layout=layout).output
-    got = rt.fp8_linear_codes(codes, scales, b, layout=layout, out_dtype=torch.bfloat16).output
-    assert torch.equal(got.float(), rounded)
+    ref = rt.execute_fp8_linear(x, b, layout=layout, f32_output=True).output.double()
+    size = rt.execute_fp8_linear(x.abs(), WideProjectionBinding(w & 0x7f, b.scale), layout=layout, f32_output=True).output
+    got = rt.fp8_linear_codes(codes, scales, b, layout=layout).output.double()
+    assert ((got - ref).abs() <= 2 * (cols / 16 + 16) * 2.0 ** -23 * 1.001 * size.double()).all()
+
+
+@pytest.mark.parametrize("width", [1, 7, 13, 33, 64, 128, 140, 256, 300, 600])
+@pytest.mark.parametrize("rows,cols", [(128, 128), (384, 640), (256, 4096), (9600, 256), (4096, 2048)])
+def test_fp8_sums_are_exact_on_small_integers(rt, width, rows, cols):
+    # codes of small integers, scales powers of two: every sum is exact in f32, every index error shows
+    from mimo_prismwing_b200.runtime import WideProjectionBinding
+    x = torch.randint(-3, 4, (width, cols), generator=gen(43), device="cuda").float()
+    w = torch.randint(-3, 4, (rows, cols), generator=gen(44), device="cuda").float()
+    xs = 2.0 ** torch.randint(-1, 2, (width, cols // 128), generator=gen(45), device="cuda").float()
+    ws = 2.0 ** torch.randint(-1, 2, (rows // 128, cols // 128), generator=gen(46), device="cuda").float()
+    b = WideProjectionBinding(w.to(torch.float8_e4m3fn).view(torch.uint8), ws)
+    out, buf = wide(torch.zeros((width, rows), device="cuda"), 5, 9.0)
+    rt.fp8_linear_codes(x.to(torch.float8_e4m3fn).view(torch.uint8), xs, b, out=out)
+    ref = (x.double() * xs.double().repeat_interleave(128, 1)) @ \
+        (w.double() * ws.double().repeat_interleave(128, 0).repeat_interleave(128, 1)).t()
+    assert torch.equal(out.double(), ref)
+    assert (buf[:, rows:] == 9.0).all()
 
 
 @pytest.mark.parametrize("act", list(ACTS))
@@ -390,10 +409,11 @@ def test_fp8_epilogue_matches_its_definition(rt, width, rows, cols, act, out):
           slack + 1e-6 * (3 + res.double().abs()))
 
 
-def test_fp8_codes_over_more_tokens_than_one_descriptor_holds(rt):
-    x, b = fp8_case(6144 + 70, 128, 128, 54)
+def test_fp8_codes_over_many_tokens(rt):
+    x, b = fp8_case(6144 + 70, 256, 128, 54)
     codes, scales = rt.quantize(x)
     ref = rt.execute_fp8_linear(x, b, f32_output=True).output
+    # one block: one product, one promotion
     assert torch.equal(rt.fp8_linear_codes(codes, scales, b).output, ref)
 
 
