@@ -48,8 +48,15 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ void arrive_remote(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrivals that hand a TMEM accumulator back to the MMA: what they order is the
+// tcgen05.ld before them (tcgen05.wait::ld and the before_thread_sync fence), no
+// memory, so they are relaxed.  (As releases they waited for the warp's stores
+// and copies each time.)
+__device__ __forceinline__ void arrive_relaxed_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_relaxed(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 __device__ __forceinline__ void store_remote4(uint32_t addr, float x, float y, float z, float w) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
@@ -91,10 +98,10 @@ __device__ __forceinline__ bool try_wait_sleep(uint64_t *bar, uint32_t parity) {
 // `abort` (shared memory) makes a CTA's other waits give up once one has.
 template <bool PAIR = false>
 __device__ __forceinline__ bool bounded_wait(volatile int *abort, uint64_t *bar, uint32_t parity, uint32_t *flags) {
-  if (*abort) return false;
   if (try_wait_sleep<PAIR>(bar, parity)) return true;
   const uint64_t start = global_timer_ns();
   do {
+    if (*abort) return false;
     if (try_wait_sleep<PAIR>(bar, parity)) return true;
   } while (global_timer_ns() - start <= kWaitLimitNs);
   *abort = 1;
@@ -189,22 +196,26 @@ uint32_t clusters_at_once(uint32_t cluster, uint32_t threads, uint32_t smem, int
   return (uint32_t)n;
 }
 
-// K splits of `tiles` tiles: the count with the least time over waves of
-// clusters.  A k-block takes about 512 cycles either way (a pair's products; a
-// tile's operands through L2), a wave 4000 more, with the exchange 8000.  Every
-// split keeps four k-blocks.
+// A tile kernel's time in cycles: per column block, and per wave of tiles
+// without and with the exchange of K splits.
+struct TileCost {
+  uint32_t block, wave, wave_split;
+};
+struct Splits {
+  uint32_t n;
+  uint64_t cost;
+};
+
+// K splits of `tiles` tiles: the count with the least time over the waves of
+// clusters.  Every split keeps four column blocks.
 template <auto Kernel>
-uint32_t best_splits(uint64_t tiles, uint32_t k_blocks, uint32_t most, uint32_t cta_per_split, uint32_t threads,
-                     uint32_t smem, int num_sms) {
-  uint32_t best = 1u;
-  uint64_t least = ~(uint64_t)0;
+Splits best_splits(const TileCost &t, uint64_t tiles, uint32_t k_blocks, uint32_t most, uint32_t cta_per_split,
+                   uint32_t threads, uint32_t smem, int num_sms) {
+  Splits best{1u, ~(uint64_t)0};
   for (uint32_t s = 1u; s <= most && (s == 1u || s * 4u <= k_blocks); ++s) {
     const uint64_t n = clusters_at_once<Kernel>(s * cta_per_split, threads, smem, num_sms);
-    const uint64_t waves = (tiles + n - 1u) / n, cost = waves * ((uint64_t)k_blocks * 512u / s + (s > 1u ? 8000u : 4000u));
-    if (cost < least) {
-      least = cost;
-      best = s;
-    }
+    const uint64_t cost = (tiles + n - 1u) / n * ((uint64_t)k_blocks * t.block / s + (s > 1u ? t.wave_split : t.wave));
+    if (cost < best.cost) best = {s, cost};
   }
   return best;
 }

@@ -132,52 +132,105 @@ __device__ __forceinline__ void activate_all(float (&v)[N], uint32_t act) {
   }
 }
 
-// The epilogue of four consecutive columns c .. c + 3 (c % 4 == 0) of token t,
-// with one access per array where its rows allow.  False when a stored value
-// is not finite.
-__device__ __forceinline__ bool finish4(const EpilogueArgs &e, float4 q, float4 bias, uint64_t t, uint32_t c) {
-  float v[4] = {q.x + bias.x, q.y + bias.y, q.z + bias.z, q.w + bias.w};
-  activate_all(v, e.act);
-  const uint32_t rz = e.residual_dtype == PW_DTYPE_F32 ? 4u : 2u, yz = e.y_dtype == PW_DTYPE_F32 ? 4u : 2u;
-  if (e.residual) {
-    const uint8_t *p = static_cast<const uint8_t *>(e.residual) + (t * e.residual_stride + c) * rz;
-    if ((reinterpret_cast<uintptr_t>(p) & (4u * rz - 1u)) == 0u) {
-      if (rz == 4u) {
-        const float4 r = *reinterpret_cast<const float4 *>(p);
-        v[0] += r.x, v[1] += r.y, v[2] += r.z, v[3] += r.w;
-      } else {
-        const uint2 r = *reinterpret_cast<const uint2 *>(p);
-        if (e.residual_dtype == PW_DTYPE_BF16) {
-          v[0] += __uint_as_float(r.x << 16), v[1] += __uint_as_float(r.x & 0xffff0000u);
-          v[2] += __uint_as_float(r.y << 16), v[3] += __uint_as_float(r.y & 0xffff0000u);
-        } else {
-          const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&r.x));
-          const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&r.y));
-          v[0] += a.x, v[1] += a.y, v[2] += b.x, v[3] += b.y;
-        }
-      }
-    } else {
+// Whether four consecutive elements from any column c, c % 4 == 0, of these rows can
+// be accessed at once.
+__device__ __forceinline__ bool quad_access(const void *p, uint64_t stride, uint32_t dtype) {
+  const uint32_t z = dtype == PW_DTYPE_F32 ? 4u : 2u;
+  return reinterpret_cast<uintptr_t>(p) % (4u * z) == 0u && stride % 4u == 0u;
+}
+
+// R quads of four columns (column % 4 == 0) of a thread: DOWN: columns c .. c + 3 of
+// the tokens t0 + 8 j with 8 j < n; else columns c + 4 j .. of token t0, n ignored.
+template <int R, bool DOWN>
+struct Quads {
+  uint64_t t0;
+  uint32_t c, n;
+  __device__ __forceinline__ bool in(uint32_t j) const { return !DOWN || 8u * j < n; }
+  __device__ __forceinline__ uint64_t at(uint32_t j, uint64_t stride) const {
+    return DOWN ? (t0 + 8u * j) * stride + c : t0 * stride + c + 4u * j;
+  }
+};
+
+// Their residual: loads only, all in flight, so they can be issued before what
+// they are added to is ready (past the end: the first quad again).
+template <int R, bool DOWN>
+__device__ __forceinline__ void load_quads(const EpilogueArgs &e, const Quads<R, DOWN> &g, bool quad_residual,
+                                           uint32_t (&raw)[R][4]) {
+  if (!quad_residual) {
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) v[i] += load_elem(e.residual, t * e.residual_stride + c + i, e.residual_dtype);
+    for (uint32_t j = 0; j < R; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        raw[j][i] =
+            __float_as_uint(load_elem(e.residual, g.at(g.in(j) ? j : 0u, e.residual_stride) + i, e.residual_dtype));
+  } else if (e.residual_dtype == PW_DTYPE_F32) {
+#pragma unroll
+    for (uint32_t j = 0; j < R; ++j) {
+      const uint4 q = *reinterpret_cast<const uint4 *>(static_cast<const uint32_t *>(e.residual) +
+                                                       g.at(g.in(j) ? j : 0u, e.residual_stride));
+      raw[j][0] = q.x, raw[j][1] = q.y, raw[j][2] = q.z, raw[j][3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < R; ++j) {
+      const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(e.residual) +
+                                                       g.at(g.in(j) ? j : 0u, e.residual_stride));
+      raw[j][0] = q.x, raw[j][1] = q.y, raw[j][2] = raw[j][3] = 0u;
+    }
+  }
+}
+
+// Their epilogue.  False when a stored value is not finite.
+template <int R, bool DOWN>
+__device__ __forceinline__ bool finish_quads(const EpilogueArgs &e, const Quads<R, DOWN> &g, float (&v)[4 * R],
+                                             const float4 (&bias)[DOWN ? 1 : R], const uint32_t (&raw)[R][4],
+                                             bool quad_residual, bool quad_y) {
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const float4 b = bias[DOWN ? 0 : j];
+    v[4 * j] += b.x, v[4 * j + 1] += b.y, v[4 * j + 2] += b.z, v[4 * j + 3] += b.w;
+  }
+  activate_all(v, e.act);
+  if (e.residual) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      float r[4];
+      if (!quad_residual || e.residual_dtype == PW_DTYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = __uint_as_float(raw[j][i]);
+      } else if (e.residual_dtype == PW_DTYPE_BF16) {
+        r[0] = __uint_as_float(raw[j][0] << 16), r[1] = __uint_as_float(raw[j][0] & 0xffff0000u);
+        r[2] = __uint_as_float(raw[j][1] << 16), r[3] = __uint_as_float(raw[j][1] & 0xffff0000u);
+      } else {
+        const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&raw[j][0]));
+        const float2 hi = __half22float2(*reinterpret_cast<const __half2 *>(&raw[j][1]));
+        r[0] = lo.x, r[1] = lo.y, r[2] = hi.x, r[3] = hi.y;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * j + i] += r[i];
     }
   }
   uint32_t top = 0u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  uint8_t *p = static_cast<uint8_t *>(e.y) + (t * e.y_stride + c) * yz;
-  if ((reinterpret_cast<uintptr_t>(p) & (4u * yz - 1u)) == 0u) {
-    if (yz == 4u) {
-      *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    } else if (e.y_dtype == PW_DTYPE_BF16) {
-      *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2_rn(v[0], v[1]), pack_bf16x2_rn(v[2], v[3]));
-    } else {
-      const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-      *reinterpret_cast<uint2 *>(p) =
-          make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
-    }
-  } else {
+  for (uint32_t j = 0; j < R; ++j) {
+    if (!g.in(j)) continue;
+    const float *q = v + 4 * j;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) store_elem(e.y, t * e.y_stride + c + i, e.y_dtype, v[i]);
+    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(q[i]) & 0x7fffffffu);
+    const uint64_t at = g.at(j, e.y_stride);
+    if (!quad_y) {
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) store_elem(e.y, at + i, e.y_dtype, q[i]);
+    } else if (e.y_dtype == PW_DTYPE_F32) {
+      *reinterpret_cast<float4 *>(static_cast<float *>(e.y) + at) = make_float4(q[0], q[1], q[2], q[3]);
+    } else if (e.y_dtype == PW_DTYPE_BF16) {
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(e.y) + at) =
+          make_uint2(pack_bf16x2_rn(q[0], q[1]), pack_bf16x2_rn(q[2], q[3]));
+    } else {
+      const __half2 lo = __floats2half2_rn(q[0], q[1]), hi = __floats2half2_rn(q[2], q[3]);
+      *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(e.y) + at) =
+          make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+    }
   }
   return top < overflow_bits(e.y_dtype);
 }

@@ -4,12 +4,13 @@
 // Tokens are the TMEM lanes (A), weight rows the columns (B): a thread then has
 // one token, whose scale of a column block is one value, and the weight scale is
 // one value for the 64 or 128 columns that a warp reads, so promoting a block is
-// acc += d * (S xs) with packed FMAs.  Every 128-column block gets a fresh
+// acc += d * (S xs).  (Packed FMAs, two values per instruction, were slower: 45 cycles
+// for a warp's 32 values against 36.)  Every 128-column block gets a fresh
 // accumulator (the checkpoint's f32 scales are not powers of two, which the
 // hardware block scaling would need), so the epilogue warps read 128 x columns of
 // TMEM per block while the MMA warp fills the next accumulator.
 //
-//  * PAIR, for more than 128 tokens: two CTAs on a 256-token x 256-row tile
+//  * PAIR, for many tokens: two CTAs on a 256-token x 256-row tile
 //    (cta_group::2), 128 tokens of each CTA's own and half of the weight rows
 //    each.  A 128 x 128 tile of one CTA needs 8 KB of operands from shared memory
 //    per 64 cycles of products, all that shared memory gives, before TMA has
@@ -17,7 +18,7 @@
 //    sums per thread: setmaxnreg moves the registers of the other four to them.
 //    One token takes 128 sums x 32 blocks of promotion, so the pipe that bounds
 //    this kernel is the epilogue's FMAs and TMEM reads together with the MMAs.
-//  * one CTA, up to 128 tokens: 128 x 128 tiles, bound by the weight stream.  When
+//  * one CTA, for the widths between: 128 x 128 tiles, bound by the weight stream.  When
 //    the tiles are fewer than the SMs a cluster's CTAs split K and exchange their
 //    sums (pw_cluster.cuh).
 #include <cstdint>
@@ -46,9 +47,14 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint32_t kSmemLimit = 227u * 1024u;
 constexpr uint32_t kMaxBlocks = 32;   // K <= 4096
+// Measured cycles (256 or more tokens of 4096 columns, B200 at 1.9 GHz): the one-CTA
+// tile 900 per block and 10000 per wave, a pair's, of four times the products, 1000
+// and 21000.  They meet at 512 tokens of [4096, 4096] (23.4 and 24.8 us); 1024
+// tokens take 44 and 31 us, 203 of [4096, 2048] 11.8 and 16.2 us.
+constexpr TileCost kCostOne{900u, 10000u, 12000u}, kCostPair{1000u, 21000u, 26000u};
 constexpr uint32_t kTokenGroup = 8;   // token tiles that neighbouring pairs share weights over
-// Register split of PAIR: 256 x 224 + 128 x 40 of the 384 x 168 at launch.
-constexpr int kRegsLaunch = 168, kRegsEpi = 224, kRegsOther = 40;
+// Register split of PAIR: 256 x 240 + 128 x 24, all of the 384 x 168 at launch.
+constexpr int kRegsLaunch = 168, kRegsEpi = 240, kRegsOther = 24;
 static_assert(kEpiWarps * 32 * kRegsEpi + kEpiWarp0 * 32 * kRegsOther <= kThreads * kRegsLaunch, "register split");
 
 template <bool PAIR>
@@ -324,6 +330,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         w1 = __ldg(a.ws + (uint64_t)s1 * kblocks + lane);
       }
     };
+    const uint32_t tempty_lead = map_rank(smem_addr(sh.tempty), lead);  // the leading CTA's
+    const bool quad_r = quad_access(a.ep.residual, a.ep.residual_stride, a.ep.residual_dtype);
+    const bool quad_y = quad_access(a.ep.y, a.ep.y_stride, a.ep.y_dtype);
     uint32_t acc_slot = 0, aphase = 0, ti = 0;
     float wn0 = 0.0f, wn1 = 0.0f;
     if (u_begin < total) {
@@ -344,48 +353,53 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       const float wc0 = wn0, wc1 = wn1;
       if (u + u_step < total) ws_load(u + u_step, wn0, wn1);
 
-      float2 acc[CH][16];
+      float acc[C::COLS];
 #pragma unroll
-      for (uint32_t q = 0; q < CH; ++q)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[q][i] = make_float2(0.0f, 0.0f);
+      for (uint32_t i = 0; i < C::COLS; ++i) acc[i] = 0.0f;
       if (active) {
         // A chunk of 32 columns loads while the previous one is promoted, across
         // blocks too; the accumulator goes back to the MMA once its last chunk is
-        // in registers.
+        // in registers.  The next block's scales are read a block ahead.
         float v[2][32];
+        auto scales = [&](uint32_t kb, float &s0, float &s1) {
+          const float x = xsb[kb * 32u + lane];
+          s0 = __fmul_rn(__shfl_sync(0xffffffffu, wc0, kb), x);
+          s1 = C::COLS > 64u ? __fmul_rn(__shfl_sync(0xffffffffu, wc1, kb), x) : s0;
+        };
+        float s0, s1;
+        scales(kb0, s0, s1);
         bool ok = __all_sync(0xffffffffu, bounded_wait(sh.abort, &sh.tfull[acc_slot], aphase, a.flags));
         tc_fence_after();
         tc::tmem_ld32(cols + acc_slot * BN, v[0]);
         tc::tmem_wait_ld(v[0]);
 #pragma unroll 1
         for (uint32_t kb = kb0; kb < kb1; ++kb) {
-          const float x = xsb[kb * 32u + lane];
-          const float s0 = ok ? __fmul_rn(__shfl_sync(0xffffffffu, wc0, kb), x) : 0.0f;
-          const float s1 = C::COLS > 64u ? (ok ? __fmul_rn(__shfl_sync(0xffffffffu, wc1, kb), x) : 0.0f) : s0;
+          if (!ok) s0 = s1 = 0.0f;
+          const bool more = kb + 1u < kb1;
+          float n0 = 0.0f, n1 = 0.0f;
 #pragma unroll
           for (uint32_t q = 0; q < CH; ++q) {
             const float s = q < 2u ? s0 : s1;
-            const float2 s2 = make_float2(s, s);
             float(&now)[32] = v[q & 1u];
             float(&next)[32] = v[(q & 1u) ^ 1u];
             bool load = true;
             if (q + 1u < CH) {
               tc::tmem_ld32(cols + acc_slot * BN + 32u * (q + 1u), next);
+              if (q == 0u && more) scales(kb + 1u, n0, n1);
             } else {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) {
                 if (PAIR)
-                  arrive_remote(map_rank(smem_addr(&sh.tempty[acc_slot]), lead));
+                  arrive_relaxed_remote(tempty_lead + acc_slot * 8u);
                 else
-                  mbar_arrive(&sh.tempty[acc_slot]);
+                  arrive_relaxed(&sh.tempty[acc_slot]);
               }
               if (++acc_slot == NACC) {
                 acc_slot = 0;
                 aphase ^= 1u;
               }
-              load = kb + 1u < kb1;
+              load = more;
               if (load) {
                 ok = __all_sync(0xffffffffu, bounded_wait(sh.abort, &sh.tfull[acc_slot], aphase, a.flags));
                 tc_fence_after();
@@ -393,10 +407,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
               }
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              acc[q][i] = __ffma2_rn(make_float2(now[2 * i], now[2 * i + 1]), s2, acc[q][i]);
+            for (int i = 0; i < 32; ++i) acc[32u * q + i] = __fmaf_rn(now[i], s, acc[32u * q + i]);
             if (load) tc::tmem_wait_ld(next);
           }
+          s0 = n0;
+          s1 = n1;
         }
       } else {
         // no tokens or no rows here: keep the accumulators' handshake
@@ -407,9 +422,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
           __syncwarp();
           if (lane == 0) {
             if (PAIR)
-              arrive_remote(map_rank(smem_addr(&sh.tempty[acc_slot]), lead));
+              arrive_relaxed_remote(tempty_lead + acc_slot * 8u);
             else
-              mbar_arrive(&sh.tempty[acc_slot]);
+              arrive_relaxed(&sh.tempty[acc_slot]);
           }
           if (++acc_slot == NACC) {
             acc_slot = 0;
@@ -424,23 +439,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         cluster_sync_all();  // every CTA's MMAs have read their last stage
         if (active) {
 #pragma unroll
-          for (uint32_t q = 0; q < CH; ++q)
-            x.send32(reinterpret_cast<const float(&)[32]>(acc[q]), col0 + 32u * q, row);
+          for (uint32_t q = 0; q < CH; ++q) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = acc[32u * q + i];
+            x.send32(v, col0 + 32u * q, row);
+          }
         }
-        __syncwarp();
-        cluster_sync_all();  // every CTA's sums have arrived
         const uint32_t first = x.split * x.share, mid = x.share / 2u & ~7u;
         const uint32_t in_tile = first < x.cols ? min(x.share, x.cols - first) : 0u;
+        // this thread's token, columns [begin, end) of the share, eight at a time
+        // (rows are a multiple of 64), their residual and bias one step ahead
         const uint32_t begin = half ? mid : 0u, end = half ? in_tile : min(mid, in_tile);
+        const bool mine = tok_q + lane < a.width;
+        Quads<2, false> g{tok_q + lane, rt * BN + first + begin, 0u};
+        uint32_t raw[2][4];
+        float4 bias[2];
+        auto fetch = [&]() {
+          bias[0] = bias4(a.ep, g.c);
+          bias[1] = bias4(a.ep, g.c + 4u);
+          if (a.ep.residual) load_quads(a.ep, g, quad_r, raw);
+        };
+        if (mine && begin < end) fetch();
+        __syncwarp();
+        cluster_sync_all();  // every CTA's sums have arrived
         bool ok = true;
-        if (tok_q + lane < a.width)
+        if (mine)
 #pragma unroll 1
-          for (uint32_t b = begin; b < end; b += 8u) {  // rows are a multiple of 64: whole eights
+          for (uint32_t b = begin; b < end; b += 8u) {
+            const Quads<2, false> now = g;
+            uint32_t cur[2][4];
+            float4 cur_bias[2] = {bias[0], bias[1]};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) cur[i / 4][i % 4] = raw[i / 4][i % 4];
+            g.c += 8u;
+            if (b + 8u < end) fetch();
             float v[8];
             x.receive8(v, b, row);
-            const uint32_t c = rt * BN + first + b;
-            ok = finish4(a.ep, make_float4(v[0], v[1], v[2], v[3]), bias4(a.ep, c), tok_q + lane, c) && ok;
-            ok = finish4(a.ep, make_float4(v[4], v[5], v[6], v[7]), bias4(a.ep, c + 4u), tok_q + lane, c + 4u) && ok;
+            ok = finish_quads(a.ep, now, v, cur_bias, cur, quad_r, quad_y) && ok;
           }
         if (!ok) raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
       } else {
@@ -448,27 +484,48 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         // quarter no longer needs once both of its warps are past the last block:
         // 16 columns at a time, a 64-byte row per token (16-byte chunk i at
         // position i ^ ((token >> 1) & 3), so that neither side conflicts), then
-        // four columns per thread, coalesced.
+        // four columns of a few tokens per thread, coalesced.  The loop is rolled
+        // (the sums move down 16 registers per turn): unrolled, its code left the
+        // instruction cache and a tile's epilogue took as long as its products.
+        // lane l loads the bias of the warp's columns 4 l .. 4 l + 3
+        float4 biasc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (active && 4u * lane < C::COLS) biasc = bias4(a.ep, c_base + 4u * lane);
         named_bar_sync(2u + quarter, 64u);
         if (active) {
           uint8_t *stg = reinterpret_cast<uint8_t *>(xsb) + half * 2048u;
+          const uint32_t c4 = lane % 4u, r0 = lane / 4u;
           bool ok = true;
-#pragma unroll
+#pragma unroll 1
           for (uint32_t h = 0; h < C::COLS / 16u; ++h) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-              const float2 lo = acc[h / 2u][8u * (h % 2u) + 2u * i], hi = acc[h / 2u][8u * (h % 2u) + 2u * i + 1u];
+            for (uint32_t i = 0; i < 4; ++i)
               *reinterpret_cast<float4 *>(stg + lane * 64u + ((i ^ ((lane >> 1) & 3u)) << 4)) =
-                  make_float4(lo.x, lo.y, hi.x, hi.y);
+                  make_float4(acc[4u * i], acc[4u * i + 1u], acc[4u * i + 2u], acc[4u * i + 3u]);
+            __syncwarp();
+            const uint32_t col = c_base + h * 16u + c4 * 4u;
+            const uint32_t from = h * 4u + c4;
+            const float4 bias[1] = {
+                make_float4(__shfl_sync(0xffffffffu, biasc.x, from), __shfl_sync(0xffffffffu, biasc.y, from),
+                            __shfl_sync(0xffffffffu, biasc.z, from), __shfl_sync(0xffffffffu, biasc.w, from))};
+            // a pair's thread has registers for its four tokens at once
+            constexpr uint32_t R = PAIR ? 4u : 2u;
+#pragma unroll 1
+            for (uint32_t r = r0; r < rows_here; r += 8u * R) {
+              const Quads<R, true> g{tok_q + r, col, rows_here - r};
+              uint32_t raw[R][4];
+              if (a.ep.residual) load_quads(a.ep, g, quad_r, raw);
+              float q[4u * R];
+#pragma unroll
+              for (uint32_t j = 0; j < R; ++j) {
+                const uint32_t rj = r + 8u * j;
+                const float4 f = *reinterpret_cast<const float4 *>(stg + rj * 64u + ((c4 ^ ((rj >> 1) & 3u)) << 4));
+                q[4u * j] = f.x, q[4u * j + 1u] = f.y, q[4u * j + 2u] = f.z, q[4u * j + 3u] = f.w;
+              }
+              ok = finish_quads(a.ep, g, q, bias, raw, quad_r, quad_y) && ok;
             }
             __syncwarp();
-            const uint32_t c = lane % 4u, col = c_base + h * 16u + c * 4u;
-            const float4 bias = bias4(a.ep, col);
-#pragma unroll 1
-            for (uint32_t r = lane / 4u; r < rows_here; r += 8u) {
-              const float4 q = *reinterpret_cast<const float4 *>(stg + r * 64u + ((c ^ ((r >> 1) & 3u)) << 4));
-              ok = finish4(a.ep, q, bias, tok_q + r, col) && ok;
-            }
+#pragma unroll
+            for (uint32_t i = 0; i + 16u < C::COLS; ++i) acc[i] = acc[i + 16u];
             __syncwarp();
           }
           if (!ok) raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
@@ -492,50 +549,65 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
   }
 }
 
+// Tiles, column blocks and the best K split of a kernel on these sizes.
+template <bool PAIR>
+Splits plan(const Fp8CodesArgs &a, int num_sms, uint32_t &row_tiles, uint32_t &token_tiles, uint32_t &stages) {
+  using C = Cfg<PAIR>;
+  constexpr uint32_t CTAS = PAIR ? 2u : 1u, kTokens = CTAS * kTileRows;
+  row_tiles = (a.rows + C::BN - 1u) / C::BN;
+  token_tiles = (a.width + kTokens - 1u) / kTokens;
+  stages = (a.K / 128u + C::KBS - 1u) / C::KBS;
+  return best_splits<k_fp8_gemm<PAIR>>(PAIR ? kCostPair : kCostOne, (uint64_t)row_tiles * token_tiles, stages * C::KBS,
+                                       kMaxSplits / CTAS, CTAS, kThreads, C::SMEM, num_sms);
+}
+
+// Raises the kernel's shared-memory limit, without which its occupancy is none.
+template <bool PAIR>
+cudaError_t prepare() {
+  cudaError_t e = allow_smem<k_fp8_gemm<PAIR>>(Cfg<PAIR>::SMEM);
+  if (e != cudaSuccess || !PAIR) return e;
+  // the register split must fit what the launch allocates, or setmaxnreg would wait for good
+  static std::atomic<int> regs{0};
+  if (regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes at;
+    if ((e = cudaFuncGetAttributes(&at, k_fp8_gemm<PAIR>)) != cudaSuccess) return e;
+    regs.store(at.numRegs, std::memory_order_relaxed);
+  }
+  return regs.load(std::memory_order_relaxed) < kRegsLaunch ? cudaErrorInvalidConfiguration : cudaSuccess;
+}
+
 template <bool PAIR>
 cudaError_t launch_one(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream) {
   using C = Cfg<PAIR>;
-  constexpr auto kernel = k_fp8_gemm<PAIR>;
-  cudaError_t e = allow_smem<k_fp8_gemm<PAIR>>(C::SMEM);
-  if (e != cudaSuccess) return e;
-  if (PAIR) {
-    // the register split must fit what the launch allocates, or setmaxnreg would wait for good
-    static std::atomic<int> regs{0};
-    if (regs.load(std::memory_order_relaxed) == 0) {
-      cudaFuncAttributes at;
-      if ((e = cudaFuncGetAttributes(&at, kernel)) != cudaSuccess) return e;
-      regs.store(at.numRegs, std::memory_order_relaxed);
-    }
-    if (regs.load(std::memory_order_relaxed) < kRegsLaunch) return cudaErrorInvalidConfiguration;
-  }
+  constexpr uint32_t CTAS = PAIR ? 2u : 1u;
   Args A{};
   A.a = a;
+  A.splits = plan<PAIR>(a, num_sms, A.row_tiles, A.token_tiles, A.stages).n;
   const bool qkv = a.layout != PW_LAYOUT_PLAIN;
   // up to 128 tokens a stage loads whole 32-token chunks of them
-  A.box_tokens = PAIR ? 128u : (a.width + 31u) / 32u * 32u;
+  A.box_tokens = a.width > 96u ? 128u : (a.width + 31u) / 32u * 32u;
   if (!encode_weight_map(&A.wmap, a.w, a.rows, a.K, qkv ? 64u : 128u, qkv ? 1u : C::KBS) ||
       !encode_weight_map(&A.xmap, a.codes, a.width, a.K, A.box_tokens, C::KBS))
     return cudaErrorInvalidValue;
-  constexpr uint32_t kTokens = PAIR ? 256u : 128u;
-  A.row_tiles = (a.rows + C::BN - 1u) / C::BN;
-  A.token_tiles = (a.width + kTokens - 1u) / kTokens;
-  A.stages = (a.K / 128u + C::KBS - 1u) / C::KBS;
-  const uint64_t tiles = (uint64_t)A.row_tiles * A.token_tiles;
+  const uint64_t tiles = (uint64_t)A.row_tiles * A.token_tiles, at_once = (uint64_t)num_sms / CTAS;
   if (tiles > 0x7fffffffull / kMaxSplits) return cudaErrorInvalidValue;
-  constexpr uint32_t CTAS = PAIR ? 2u : 1u;
-  A.splits = best_splits<k_fp8_gemm<PAIR>>(tiles, A.stages * C::KBS, kMaxSplits / CTAS, CTAS, kThreads, C::SMEM, num_sms);
-  const uint64_t at_once = (uint64_t)num_sms / CTAS;
   const uint32_t clusters = (uint32_t)(A.splits > 1u ? tiles * A.splits : tiles < at_once ? tiles : at_once);
   Launch l(CTAS * clusters, kThreads, CTAS * A.splits, C::SMEM, stream);
-  e = cudaLaunchKernelEx(&l.cfg, kernel, A);
+  cudaError_t e = cudaLaunchKernelEx(&l.cfg, k_fp8_gemm<PAIR>, A);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 }  // namespace fp8g
 
 cudaError_t launch_fp8_gemm(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream) {
-  if (a.width == 0 || a.rows % 64u || a.K == 0 || a.K % 128u || a.K > 128u * fp8g::kMaxBlocks) return cudaErrorInvalidValue;
-  return a.width <= 128u ? fp8g::launch_one<false>(a, num_sms, stream) : fp8g::launch_one<true>(a, num_sms, stream);
+  using namespace fp8g;
+  if (a.width == 0 || a.rows % 64u || a.K == 0 || a.K % 128u || a.K > 128u * kMaxBlocks) return cudaErrorInvalidValue;
+  cudaError_t e;
+  if ((e = prepare<false>()) != cudaSuccess || (e = prepare<true>()) != cudaSuccess) return e;
+  uint32_t r, t, s;
+  if (a.width <= 128u || plan<false>(a, num_sms, r, t, s).cost <= plan<true>(a, num_sms, r, t, s).cost)
+    return launch_one<false>(a, num_sms, stream);
+  return launch_one<true>(a, num_sms, stream);
 }
 
 }  // namespace pw

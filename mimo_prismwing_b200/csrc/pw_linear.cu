@@ -53,6 +53,9 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr uint32_t kBlockK = 64;        // columns of a k-block: one 128-byte line
 constexpr uint32_t kSmemLimit = 227u * 1024u;
+// A 64-column block takes about 512 cycles in either kernel (a pair's products; a
+// tile's operands through L2).
+constexpr TileCost kCost{512u, 4000u, 8000u};
 constexpr uint32_t kTokenGroup = 8;     // token tiles that neighbouring CTAs share weights over
 
 template <int BN>
@@ -393,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tile(const __grid_consta
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.tempty[acc]);
+        if (lane == 0) arrive_relaxed(&sh.tempty[acc]);
         if (++acc == NACC) {
           acc = 0;
           aphase ^= 1u;
@@ -613,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_pair(const __grid_consta
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_remote(map_rank(smem_addr(&sh.tempty[acc]), lead));
+      if (lane == 0) arrive_relaxed_remote(map_rank(smem_addr(&sh.tempty[acc]), lead));
       if (++acc == 2u) {
         acc = 0;
         aphase ^= 1u;
@@ -660,7 +663,7 @@ cudaError_t launch_tile(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   cudaError_t e = allow_smem<k_linear_tile<BN>>(C::SMEM);
   if (e != cudaSuccess) return e;
   const uint32_t tiles = A.row_tiles * A.token_tiles, sms = (uint32_t)num_sms;
-  A.splits = best_splits<k_linear_tile<BN>>(tiles, A.stages * C::KBS, kMaxSplits, 1u, kThreads, C::SMEM, num_sms);
+  A.splits = best_splits<k_linear_tile<BN>>(kCost, tiles, A.stages * C::KBS, kMaxSplits, 1u, kThreads, C::SMEM, num_sms).n;
   Launch l(A.splits > 1u ? tiles * A.splits : tiles < sms ? tiles : sms, kThreads, A.splits, C::SMEM, stream);
   e = cudaLaunchKernelEx(&l.cfg, k_linear_tile<BN>, A);
   return e != cudaSuccess ? e : cudaGetLastError();
@@ -673,7 +676,7 @@ cudaError_t launch_pair(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   cudaError_t e = allow_smem<k_linear_pair>(C::SMEM);
   if (e != cudaSuccess) return e;
   const uint32_t tiles = A.row_tiles * A.token_tiles, pairs = (uint32_t)num_sms / 2u;
-  A.splits = best_splits<k_linear_pair>(tiles, A.stages, kMaxSplits / 2u, 2u, kThreads, C::SMEM, num_sms);
+  A.splits = best_splits<k_linear_pair>(kCost, tiles, A.stages, kMaxSplits / 2u, 2u, kThreads, C::SMEM, num_sms).n;
   Launch l(2u * (A.splits > 1u ? tiles * A.splits : tiles < pairs ? tiles : pairs), kThreads, 2u * A.splits, C::SMEM, stream);
   e = cudaLaunchKernelEx(&l.cfg, k_linear_pair, A);
   return e != cudaSuccess ? e : cudaGetLastError();
