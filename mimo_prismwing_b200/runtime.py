@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -198,6 +199,7 @@ class WideMoeRuntime:
         self.fused_gate_up = fused_gate_up
         self._banks = []
         self._bank_refs = []
+        self._init_args()
 
     # reference constructors (src/wide_metal_moe.rs:165-171)
     @classmethod
@@ -414,9 +416,19 @@ class WideMoeRuntime:
 
     # ------------------------------------- residual, norm, linear layers
     # These calls take a few microseconds on the device for a single token, so
-    # their host side is kept short: one check per tensor, no conversions.
-    def _rows(self, t: torch.Tensor, name: str, where: int) -> Rows:
-        """pw_rows of a 2-D tensor whose rows are contiguous, on device `where` (-1: the host)."""
+    # their host side is kept short: one check per tensor, and the descriptors
+    # (the structures above) packed at once into a block that the runtime keeps
+    # (like the runtime's other state, it serves one call at a time).
+    _NORM_ARGS = struct.Struct("=QIIf4x" + "QQII" * 4)       # Norm, then Rows of x, residual, sum, y
+    _LINEAR_ARGS = struct.Struct("=QQIIII" + "QQII" + "QIIQQII" + "QQII")  # Dense, Rows of x, Epilogue, Rows of y
+    _CODES_ARGS = struct.Struct("=QIIQQII" + "QQII")         # Epilogue, Rows of y
+
+    def _init_args(self) -> None:
+        self._args = ctypes.create_string_buffer(256)
+        self._args_at = ctypes.addressof(self._args)
+
+    def _rows(self, t: torch.Tensor, name: str, where: int):
+        """(data, stride, dtype) of a 2-D tensor whose rows are contiguous, on device `where` (-1: the host)."""
         shape, code = t.shape, DTYPES.get(t.dtype)
         if len(shape) == 2 and code is not None and t.get_device() == where:
             rows, cols = shape
@@ -424,7 +436,7 @@ class WideMoeRuntime:
             if rows <= 1:  # one row may have any stride in torch
                 stride = 0
             if (step == 1 or cols <= 1) and (stride >= cols or not stride and rows <= 1):
-                return Rows(t.data_ptr(), stride, code, 0)
+                return t.data_ptr(), stride, code
         if code is None:
             raise PrismwingError(-1, f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
         if t.get_device() != where:
@@ -466,66 +478,72 @@ class WideMoeRuntime:
         float32, bfloat16 or float16; weight a CUDA [hidden] of any of them.  in_place writes s over residual."""
         x = self._input(x)
         where = self._where(x)
-        xr = self._rows(x, "x", where)
+        x_at, x_stride, dt = self._rows(x, "x", where)
         T, H = x.shape
         dtype, dev = x.dtype, x.device
         if weight.dtype not in DTYPES:
             raise PrismwingError(-1, f"norm weight must be float32, bfloat16 or float16, not {weight.dtype}")
-        norm = Norm(self._vector(weight, "norm weight", H), H, DTYPES[weight.dtype], epsilon)
+        w_at = self._vector(weight, "norm weight", H)
         mem, st = self._mem(where, asynchronous)
-        ref, empty = ctypes.byref, torch.empty_strided
-        rr = sr = yr = cp = sp = total = y = codes = scales = None
+        empty, at = torch.empty_strided, self._args_at
+        r_at = r_stride = s_at = s_stride = y_at = y_dt = 0
+        rp = sp = yp = cp = gp = total = y = codes = scales = None
         if residual is not None:
             residual = self._input(residual)
-            res = self._rows(residual, "residual", where)
+            r_at, r_stride, r_dt = self._rows(residual, "residual", where)
             if residual.shape != x.shape:
                 raise PrismwingError(-2, "residual must have x's shape")
-            rr = ref(res)
+            if r_dt != dt:
+                raise PrismwingError(-1, "residual must have x's dtype")
             if in_place:
-                total, sr = residual, rr
+                total, s_at, s_stride = residual, r_at, r_stride
             else:
                 total = empty((T, H), (H, 1), dtype=dtype, device=dev)
-                sr = ref(Rows(total.data_ptr(), H, xr.dtype, 0))
+                s_at, s_stride = total.data_ptr(), H
+            rp, sp = at + 48, at + 72
         if want_y:
             if out_dtype is None:
                 out_dtype = dtype
             elif out_dtype not in DTYPES:
                 raise PrismwingError(-1, f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
             y = empty((T, H), (H, 1), dtype=out_dtype, device=dev)
-            yr = ref(Rows(y.data_ptr(), H, DTYPES[out_dtype], 0))
+            y_at, y_dt, yp = y.data_ptr(), DTYPES[out_dtype], at + 96
         if want_codes:
             G = (H + 127) // 128
             codes = empty((T, H), (H, 1), dtype=torch.uint8, device=dev)
             scales = empty((T, G), (G, 1), dtype=torch.float32, device=dev)
-            cp, sp = codes.data_ptr(), scales.data_ptr()
-        status = self._L.pw_add_rms_norm(self._rt, ref(norm), ref(xr), rr, T, sr, yr, cp, sp, mem,
-                                         ref(st) if st else None)
+            cp, gp = codes.data_ptr(), scales.data_ptr()
+        self._NORM_ARGS.pack_into(self._args, 0, w_at, H, DTYPES[weight.dtype], epsilon, x_at, x_stride, dt, 0,
+                                  r_at, r_stride, dt, 0, s_at, s_stride, dt, 0, y_at, H, y_dt, 0)
+        status = self._L.pw_add_rms_norm(self._rt, at, at + 24, rp, T, sp, yp, cp, gp, mem,
+                                         ctypes.byref(st) if st else None)
         if status:
             self._check(status)
         return NormExecution(total, y, codes, scales)
 
     def _epilogue(self, where: int, dev, width: int, cols: int, bias, activation: str, residual, out_dtype, out):
-        """(pw_epilogue, pw_rows of y, y) of a linear layer over rows on device `where`."""
+        """The fields of a linear layer's pw_epilogue and of its output's pw_rows, and the output."""
         act = ACTIVATIONS.get(activation)
         if act is None:
             raise PrismwingError(-1, f"unknown activation {activation!r}")
-        ep = Epilogue(None, 0, act)
+        b_at = b_dt = r_at = r_stride = r_dt = 0
         if bias is not None:
-            ep.bias = self._vector(bias, "bias", cols)
-            ep.bias_dtype = DTYPES[bias.dtype]
+            b_at, b_dt = self._vector(bias, "bias", cols), DTYPES[bias.dtype]
         if residual is not None:
             if residual.shape != (width, cols):
                 raise PrismwingError(-2, f"residual must be [{width}, {cols}]")
-            ep.residual = self._rows(residual, "residual", where)
+            r_at, r_stride, r_dt = self._rows(residual, "residual", where)
         if out is not None:
             if out.shape != (width, cols):
                 raise PrismwingError(-2, f"out must be [{width}, {cols}]")
-            return ep, self._rows(out, "out", where), out
-        code = DTYPES.get(out_dtype)
-        if code is None:
-            raise PrismwingError(-1, f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
-        out = torch.empty_strided((width, cols), (cols, 1), dtype=out_dtype, device=dev)
-        return ep, Rows(out.data_ptr(), cols, code, 0), out
+            y_at, y_stride, y_dt = self._rows(out, "out", where)
+        else:
+            y_dt = DTYPES.get(out_dtype)
+            if y_dt is None:
+                raise PrismwingError(-1, f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+            out = torch.empty_strided((width, cols), (cols, 1), dtype=out_dtype, device=dev)
+            y_at, y_stride = out.data_ptr(), cols
+        return (b_at, b_dt, act, r_at, r_stride, r_dt, 0, y_at, y_stride, y_dt, 0), out
 
     def linear(self, x, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
                residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
@@ -537,17 +555,17 @@ class WideMoeRuntime:
         "relu", "gelu", "gelu_tanh" or "silu"."""
         x = self._input(x)
         where = self._where(x)
-        xr = self._rows(x, "x", where)
-        wr = self._rows(weight, "weight", self.device)
+        x_at, x_stride, x_dt = self._rows(x, "x", where)
+        w_at, w_stride, w_dt = self._rows(weight, "weight", self.device)
         rows, cols = weight.shape
         width, columns = x.shape
         if columns != cols:
             raise PrismwingError(-2, f"x has {columns} columns, the weight {cols}")
         mem, st = self._mem(where, asynchronous)
-        ep, yr, out = self._epilogue(where, x.device, width, rows, bias, activation, residual, out_dtype or x.dtype, out)
-        w = Dense(wr.data, wr.stride, rows, cols, wr.dtype, 0)
-        ref = ctypes.byref
-        status = self._L.pw_linear(self._rt, ref(w), ref(xr), width, ref(ep), ref(yr), mem, ref(st) if st else None)
+        fields, out = self._epilogue(where, x.device, width, rows, bias, activation, residual, out_dtype or x.dtype, out)
+        at = self._args_at
+        self._LINEAR_ARGS.pack_into(self._args, 0, w_at, w_stride, rows, cols, w_dt, 0, x_at, x_stride, x_dt, 0, *fields)
+        status = self._L.pw_linear(self._rt, at, at + 32, width, at + 56, at + 96, mem, ctypes.byref(st) if st else None)
         if status:
             self._check(status)
         if st is None:
@@ -575,10 +593,11 @@ class WideMoeRuntime:
             raise PrismwingError(-2, f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not fit a "
                                      f"[{t.rows}, {t.cols}] projection")
         mem, st = self._mem(where, asynchronous)
-        ep, yr, out = self._epilogue(where, codes.device, width, t.rows, bias, activation, residual, out_dtype, out)
-        ref = ctypes.byref
-        status = self._L.pw_fp8_linear_codes(self._rt, ref(t), layout, codes.data_ptr(), scales.data_ptr(), width,
-                                             ref(ep), ref(yr), mem, ref(st) if st else None)
+        fields, out = self._epilogue(where, codes.device, width, t.rows, bias, activation, residual, out_dtype, out)
+        at = self._args_at
+        self._CODES_ARGS.pack_into(self._args, 0, *fields)
+        status = self._L.pw_fp8_linear_codes(self._rt, ctypes.byref(t), layout, codes.data_ptr(), scales.data_ptr(), width,
+                                             at, at + 40, mem, ctypes.byref(st) if st else None)
         if status:
             self._check(status)
         if st is None:
