@@ -257,6 +257,17 @@ __global__ void __launch_bounds__(kMaxThreads, STEPS == 1 ? 3 : STEPS == 2 ? 2 :
         for (int i = 0; i < STEPS; ++i) store_step<T, VEC>(o_sum, base_of(i), lane, hidden, s[i]);
       }
     }
+    // 16-bit weights are on their way before the reduction's barrier
+    uint4 wq[STEPS];
+    if (VEC != kElements && a.w_dtype != PW_NORM_F32) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const uint32_t c = base_of(i) + lane * 8u;
+        wq[i] = VEC == kFull || c < hidden
+                    ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.weight) + c))
+                    : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
     float sq = 0.0f;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
@@ -296,7 +307,11 @@ __global__ void __launch_bounds__(kMaxThreads, STEPS == 1 ? 3 : STEPS == 2 ? 2 :
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       float w[8];
-      if (a.w_dtype == PW_NORM_F32)
+      if (VEC != kElements && a.w_dtype == PW_NORM_BF16)
+        unpack8<__nv_bfloat16>(wq[i], w);
+      else if (VEC != kElements && a.w_dtype == PW_NORM_F16)
+        unpack8<__half>(wq[i], w);
+      else if (a.w_dtype == PW_NORM_F32)
         load_step<float, VEC>(static_cast<const float *>(a.weight), base_of(i), lane, hidden, w);
       else if (a.w_dtype == PW_NORM_BF16)
         load_step<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16 *>(a.weight), base_of(i), lane, hidden, w);
@@ -414,8 +429,8 @@ template <typename T, Access VEC, int STEPS>
 cudaError_t launch_one(const AddNormArgs &a, uint32_t threads, int num_sms, cudaStream_t stream) {
   const uint32_t per_sm = resident<k_add_norm<T, VEC, STEPS>>(threads);
   uint32_t stages = 0;
-  // The ring pays when CTAs run several rows (without it the cases above took
-  // 21.5 and 204 us).  Slots share what the resident CTAs have of shared memory.
+  // The ring pays when CTAs run several rows (without it the first and last case
+  // below took 21.5 and 204 us).  Slots share what the resident CTAs have of shared memory.
   const uint32_t row_bytes = a.hidden * (uint32_t)sizeof(T) * (a.residual ? 2u : 1u);
   if (VEC != kElements && a.rows > (uint32_t)num_sms * per_sm) {
     stages = kRingBytes / per_sm / row_bytes;
@@ -439,13 +454,12 @@ cudaError_t launch_shape(const AddNormArgs &a, uint32_t steps, uint32_t threads,
 
 template <typename T, Access VEC>
 cudaError_t launch_steps(const AddNormArgs &a, int num_sms, cudaStream_t stream) {
-  // With few rows, all the threads that a row can use.  With many, several
-  // steps per thread, so that fewer threads repeat a row's reductions and
-  // scales (measured at 1 / 2 / 4 steps: 2048 x 4096 bf16 with residual and
-  // codes 19.2 / 16.5 / 17.0 us; 16384 x 8192 f16 to f16 - / 104.7 / 100.9 us,
-  // where one step needs more than 512 threads).  Element access needs twice
-  // the registers, so two steps unless the row needs four (777 x 5003 f32:
-  // 16.8 us at two, 18.9 us at four).
+  // With few rows, all the threads that a row can use.  With many, four steps per
+  // thread, so that fewer threads repeat a row's reductions and scales (measured
+  // at 2 / 4 steps: 2048 x 4096 bf16 with residual and codes 16.6 / 15.8 us, 8192
+  // rows 46.7 / 41.9 us, 16384 x 8192 f16 to f16 108.7 / 94.2 us).  Element access
+  // needs twice the registers, so two steps unless the row needs four (777 x 5003
+  // f32: 16.8 us at two, 18.9 us at four).
   const uint32_t warp_steps = (a.hidden + 255u) / 256u;  // 1..64
   const uint32_t least = warp_steps <= 16u ? 1u : warp_steps <= 32u ? 2u : 4u;
   const uint32_t best = warp_steps >= 4u && VEC != kElements ? 4u : warp_steps >= 2u ? 2u : 1u;
