@@ -316,7 +316,7 @@ int pw_rms_norm(pw_runtime *rt, const pw_norm *norm, const float *x, uint32_t ro
  * contiguous: what pw_fp8_linear_codes takes.  Unlike pw_rms_norm, which
  * reproduces the reference's sum order and its bf16 value between the two
  * products, this rounds y once and quantizes v itself; hidden is any size up
- * to 16384 (a multiple of 256 there).
+ * to 16384 (a multiple of 256 there), epsilon at least 1e-30.
  * x, residual and sum have one dtype; y has that dtype or F32.  `residual`,
  * `sum`, `y` and codes + scales (both or neither) are optional (NULL); at least
  * one of y and codes is asked for.  sum may be x or residual itself, and y may
@@ -335,8 +335,9 @@ int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const
  * has any dtype; y may be residual, not x.  Any width, rows and cols >= 1; x
  * rows that do not start at 16-byte boundaries are copied first.  `ep` may be
  * NULL.  A non-finite output is PW_ERR_NONFINITE (PW_FLAG_NONFINITE_ROUND).
- * Results do not depend on the other tokens of the call or, between widths of
- * one kernel, on the width. */
+ * A token's result does not depend on the other tokens' values, and is the same
+ * in every call of the same sizes; other sizes may add the products in another
+ * order.  Only calls that convert or copy x use the runtime's scratch. */
 int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t width, const pw_epilogue *ep,
               const pw_rows *y, uint32_t mem, pw_stats *stats);
 
@@ -345,8 +346,8 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
  * scales f32 [width, cols / 128], contiguous, y [width, rows] of any dtype.
  * Each 128-column block's product is promoted by its two scales in f32, as in
  * pw_fp8_linear; the blocks may be added in another order (a different f32
- * rounding, nothing else).  Shapes as in pw_fp8_linear; codes start at a 16-byte
- * boundary. */
+ * rounding, nothing else).  Shapes as in pw_fp8_linear; codes and weight start at
+ * 16-byte boundaries. */
 int pw_fp8_linear_codes(pw_runtime *rt, const pw_fp8_tensor *w, uint32_t layout, const uint8_t *codes,
                         const float *scales, uint32_t width, const pw_epilogue *ep, const pw_rows *y, uint32_t mem,
                         pw_stats *stats);

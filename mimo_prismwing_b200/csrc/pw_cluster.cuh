@@ -69,14 +69,13 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
-// Bounded wait (1 s) that sleeps in hardware between looks: ten warps polling in
-// a loop took a fifth of the ALU's issue slots and, under the power cap, clock
-// from the tensor pipe.  PAIR: the pair's other CTA arrives on the barrier too.
-template <bool PAIR>
-__device__ __forceinline__ bool try_wait_sleep(uint64_t *bar, uint32_t parity) {
-  constexpr uint32_t kSleepNs = 100000;  // at most; the phase's completion wakes the thread
+// One look at a barrier's phase; SLEEP: waits in hardware for up to 100 us, woken
+// by the phase's completion.  PAIR: the pair's other CTA arrives on the barrier too.
+template <bool PAIR, bool SLEEP>
+__device__ __forceinline__ bool look(uint64_t *bar, uint32_t parity) {
+  constexpr uint32_t kSleepNs = 100000;
   uint32_t done;
-  if (PAIR)
+  if (SLEEP && PAIR)
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
@@ -84,7 +83,7 @@ __device__ __forceinline__ bool try_wait_sleep(uint64_t *bar, uint32_t parity) {
         : "=r"(done)
         : "r"(smem_addr(bar)), "r"(parity), "r"(kSleepNs)
         : "memory");
-  else
+  else if (SLEEP)
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
@@ -92,17 +91,36 @@ __device__ __forceinline__ bool try_wait_sleep(uint64_t *bar, uint32_t parity) {
         : "=r"(done)
         : "r"(smem_addr(bar)), "r"(parity), "r"(kSleepNs)
         : "memory");
+  else if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
   return done != 0u;
 }
 
-// `abort` (shared memory) makes a CTA's other waits give up once one has.
+// Bounded wait (1 s) that sleeps between looks: ten warps polling in a loop took a
+// fifth of the ALU's issue slots.  The first look does not sleep (FP8 pairs at 2048 x
+// 16384 x 4096: 221 us, 224 when it did).  `abort` (shared memory) makes a CTA's other
+// waits give up once one has.
 template <bool PAIR = false>
 __device__ __forceinline__ bool bounded_wait(volatile int *abort, uint64_t *bar, uint32_t parity, uint32_t *flags) {
-  if (try_wait_sleep<PAIR>(bar, parity)) return true;
+  if (look<PAIR, false>(bar, parity)) return true;
   const uint64_t start = global_timer_ns();
   do {
     if (*abort) return false;
-    if (try_wait_sleep<PAIR>(bar, parity)) return true;
+    if (look<PAIR, true>(bar, parity)) return true;
   } while (global_timer_ns() - start <= kWaitLimitNs);
   *abort = 1;
   raise_flag(flags, PW_FLAG_WAIT_TIMEOUT);

@@ -16,8 +16,10 @@
 //    per 64 cycles of products, all that shared memory gives, before TMA has
 //    written any; a pair's needs half of that.  Eight epilogue warps hold 128
 //    sums per thread: setmaxnreg moves the registers of the other four to them.
-//    One token takes 128 sums x 32 blocks of promotion, so the pipe that bounds
-//    this kernel is the epilogue's FMAs and TMEM reads together with the MMAs.
+//    What bounds it is the hand-over of the two accumulators between MMA and
+//    epilogue (2048 x 16384 x 4096 takes 200 us; 165 with an eighth of the FMAs,
+//    191 with a quarter of the MMAs, 162 with an eighth of the output passes).
+//    Sixteen warps with 64 sums each, with the registers that leaves, took 214 us.
 //  * one CTA, for the widths between: 128 x 128 tiles, bound by the weight stream.  When
 //    the tiles are fewer than the SMs a cluster's CTAs split K and exchange their
 //    sums (pw_cluster.cuh).

@@ -910,7 +910,7 @@ int check_rows(pw_runtime *rt, const char *name, const pw_rows *in, uint32_t row
   if (out.stride == 0u) out.stride = len;
   if (out.stride < len) return fail(rt, PW_ERR_SHAPE, "%s: row stride below the row length", name);
   if (rows == 1u) out.stride = (len + 7u) & ~(uint64_t)7u;  // one row has no stride to keep
-  if (out.stride > ((uint64_t)1 << 40) || (uint64_t)rows * out.stride > ((uint64_t)1 << 48))
+  if (out.stride > ((uint64_t)1 << 48) / (rows ? rows : 1u))
     return fail(rt, PW_ERR_SHAPE, "%s: row stride out of range", name);
   if (reinterpret_cast<uintptr_t>(out.data) % elem_size(out.dtype))
     return fail(rt, PW_ERR_ARGUMENT, "%s is not aligned to its elements", name);
@@ -993,6 +993,10 @@ int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const
   if (!norm || !norm->weight) return fail(rt, PW_ERR_ARGUMENT, "norm descriptor is null");
   if (norm->weight_dtype > PW_NORM_F16) return fail(rt, PW_ERR_ARGUMENT, "unknown norm weight_dtype");
   if (!std::isfinite(norm->epsilon) || norm->epsilon <= 0.0f) return fail(rt, PW_ERR_ARGUMENT, "invalid RMSNorm epsilon");
+  // below that, f32 squares that still matter next to it would underflow
+  if (norm->epsilon < 1e-30f) return fail(rt, PW_ERR_ARGUMENT, "RMSNorm epsilon below 1e-30");
+  if (reinterpret_cast<uintptr_t>(norm->weight) % (norm->weight_dtype == PW_NORM_F32 ? 4u : 2u))
+    return fail(rt, PW_ERR_ARGUMENT, "norm weight is not aligned to its elements");
   const uint32_t H = norm->hidden;
   if (H == 0 || H > 16384u) return fail(rt, PW_ERR_SHAPE, "RMSNorm shape mismatch (hidden %u, 1 to 16384)", H);
   if (rows == 0) return fail(rt, PW_ERR_SHAPE, "RMSNorm needs at least one row");
@@ -1180,8 +1184,9 @@ int pw_fp8_linear_codes(pw_runtime *rt, const pw_fp8_tensor *w, uint32_t layout,
   if (width > (1u << 30)) return fail(rt, PW_ERR_UNSUPPORTED, "too many rows");
   if (reinterpret_cast<uintptr_t>(scales) % 4u) return fail(rt, PW_ERR_ARGUMENT, "scales are not aligned to their elements");
   const bool host = (mem & PW_MEM_HOST) != 0;
-  if (!host && reinterpret_cast<uintptr_t>(codes) % 16u)
-    return fail(rt, PW_ERR_UNSUPPORTED, "activation codes must start at a 16-byte boundary");
+  if ((!host && reinterpret_cast<uintptr_t>(codes) % 16u) || reinterpret_cast<uintptr_t>(w->weight) % 16u)
+    return fail(rt, PW_ERR_UNSUPPORTED, "activation codes and weight must start at a 16-byte boundary");
+  if (reinterpret_cast<uintptr_t>(w->scale) % 4u) return fail(rt, PW_ERR_ARGUMENT, "weight scales are not aligned to their elements");
   const uint32_t K = w->cols, N = w->rows;
   pw_rows rr{}, yr{};
   EpilogueArgs e{};

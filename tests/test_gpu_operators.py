@@ -541,6 +541,10 @@ def test_refusals(rt):
     refused(lambda: rt.fp8_linear_codes(codes.view(torch.int8), scales, b), "argument")
     refused(lambda: rt.fp8_linear_codes(codes, scales.cpu(), b), "argument")
     refused(lambda: rt.fp8_linear_codes(codes, scales, b, layout=7), "argument")
+    from mimo_prismwing_b200.runtime import WideProjectionBinding
+    refused(lambda: rt.add_rms_norm(x, n, 1e-31), "argument")
+    skew = torch.zeros(128 * 128 + 1, dtype=torch.uint8, device="cuda")[1:].view(128, 128)
+    refused(lambda: rt.fp8_linear_codes(codes, scales, WideProjectionBinding(skew, b.scale)), "unsupported")
     flat = torch.zeros(4 * 128 + 1, dtype=torch.uint8, device="cuda")
     refused(lambda: rt.fp8_linear_codes(flat[1:].view(4, 128), scales, b), "unsupported")
 
