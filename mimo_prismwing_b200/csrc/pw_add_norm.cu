@@ -194,7 +194,8 @@ __device__ __forceinline__ void fetch_row(const AddNormArgs &a, uint8_t *ring, u
 // STEPS: steps of 8 columns per thread (hidden <= 8 * STEPS * blockDim.x).
 // stages: ring slots, or 0 to load rows straight into registers.
 template <typename T, Access VEC, int STEPS>
-__global__ void __launch_bounds__(kMaxThreads, STEPS == 1 ? 3 : STEPS == 2 ? 2 : 1) k_add_norm(const AddNormArgs a, const uint32_t stages) {
+__global__ void __launch_bounds__(kMaxThreads, STEPS == 1 ? 3 : STEPS == 2 ? 2 : 1)
+    k_add_norm(const AddNormArgs a, const uint32_t stages) {
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float part[2][kMaxThreads / 32];
   __shared__ uint64_t full[kMaxStages];
@@ -465,7 +466,8 @@ cudaError_t launch_steps(const AddNormArgs &a, int num_sms, cudaStream_t stream)
   const uint32_t best = warp_steps >= 4u && VEC != kElements ? 4u : warp_steps >= 2u ? 2u : 1u;
   const uint32_t steps = a.rows <= 2u * (uint32_t)num_sms || best < least ? least : best;
   const uint32_t threads = (warp_steps + steps - 1u) / steps * 32u;
-  if (VEC == kVectors && a.hidden == threads * 8u * steps) return launch_shape<T, kFull>(a, steps, threads, num_sms, stream);
+  if (VEC == kVectors && a.hidden == threads * 8u * steps)
+    return launch_shape<T, kFull>(a, steps, threads, num_sms, stream);
   return launch_shape<T, VEC>(a, steps, threads, num_sms, stream);
 }
 

@@ -80,6 +80,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) k_fp8_narrow(con
         wb[j][h] = in ? ldg_stream(w1 + c) : make_uint4(0u, 0u, 0u, 0u);
       }
     }
+    // codes and scales are the previous kernel's output, which it may still write while
+    // this kernel is resident: ordinary loads, not ones of read-only data
 #pragma unroll
     for (uint32_t j = 0; j < DEEP; ++j) {
       const bool in = k0 + j < kblocks;
@@ -89,13 +91,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) k_fp8_narrow(con
         const uint32_t tok = g + 8u * n;
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h)
-          xv[j][n][h] = in && tok < a.width ? __ldg(reinterpret_cast<const uint4 *>(
-                                                  a.codes + (uint64_t)tok * a.K + (k0 + j) * 128u + 64u * h + t * 16u))
+          xv[j][n][h] = in && tok < a.width ? *reinterpret_cast<const uint4 *>(
+                                                  a.codes + (uint64_t)tok * a.K + (k0 + j) * 128u + 64u * h + t * 16u)
                                             : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
           const uint32_t ot = 8u * n + 2u * t + i;
-          xs[j][n][i] = in && ot < a.width ? __ldg(a.scales + (uint64_t)ot * kblocks + k0 + j) : 0.0f;
+          xs[j][n][i] = in && ot < a.width ? a.scales[(uint64_t)ot * kblocks + k0 + j] : 0.0f;
         }
       }
     }

@@ -296,7 +296,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_tile(const __grid_consta
             } else {
 #pragma unroll
               for (int j = 0; j < (int)C::KBS; ++j) {
-                tc::tma_load_3d(dst + j * (kTileRows * 128u), &A.wmap, (kb + j) * (int)kBlockK, row0, 0, &sh.full[slot]);
+                tc::tma_load_3d(dst + j * (kTileRows * 128u), &A.wmap, (kb + j) * (int)kBlockK, row0, 0,
+                                &sh.full[slot]);
                 tc::tma_load_3d(dst + C::A_BYTES + j * (BN * 128u), &A.xmap, (kb + j) * (int)kBlockK, tok0, 0,
                                 &sh.full[slot]);
               }
@@ -490,7 +491,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_linear_pair(const __grid_consta
   const uint32_t tmem = *sh.tmem_base;
   // a cluster takes a tile; with K splits only one (the exchange reuses the ring)
   const uint32_t splits = A.splits, split = cta / 2u;
-  const uint32_t total = A.row_tiles * A.token_tiles, u_begin = blockIdx.x / (2u * splits), u_step = gridDim.x / (2u * splits);
+  const uint32_t total = A.row_tiles * A.token_tiles;
+  const uint32_t u_begin = blockIdx.x / (2u * splits), u_step = gridDim.x / (2u * splits);
   const uint32_t kb0 = A.stages * split / splits, kb1 = A.stages * (split + 1u) / splits;
 
   if (warp == (uint32_t)kProducerWarp) {
@@ -664,7 +666,8 @@ cudaError_t launch_tile(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   cudaError_t e = allow_smem<k_linear_tile<BN>>(C::SMEM);
   if (e != cudaSuccess) return e;
   const uint32_t tiles = A.row_tiles * A.token_tiles, sms = (uint32_t)num_sms;
-  A.splits = best_splits<k_linear_tile<BN>>(kCost, tiles, A.stages * C::KBS, kMaxSplits, 1u, kThreads, C::SMEM, num_sms).n;
+  A.splits =
+      best_splits<k_linear_tile<BN>>(kCost, tiles, A.stages * C::KBS, kMaxSplits, 1u, kThreads, C::SMEM, num_sms).n;
   Launch l(A.splits > 1u ? tiles * A.splits : tiles < sms ? tiles : sms, kThreads, A.splits, C::SMEM, stream);
   e = cudaLaunchKernelEx(&l.cfg, k_linear_tile<BN>, A);
   return e != cudaSuccess ? e : cudaGetLastError();
@@ -678,7 +681,8 @@ cudaError_t launch_pair(const LinearArgs &a, int num_sms, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const uint32_t tiles = A.row_tiles * A.token_tiles, pairs = (uint32_t)num_sms / 2u;
   A.splits = best_splits<k_linear_pair>(kCost, tiles, A.stages, kMaxSplits / 2u, 2u, kThreads, C::SMEM, num_sms).n;
-  Launch l(2u * (A.splits > 1u ? tiles * A.splits : tiles < pairs ? tiles : pairs), kThreads, 2u * A.splits, C::SMEM, stream);
+  Launch l(2u * (A.splits > 1u ? tiles * A.splits : tiles < pairs ? tiles : pairs), kThreads, 2u * A.splits, C::SMEM,
+           stream);
   e = cudaLaunchKernelEx(&l.cfg, k_linear_pair, A);
   return e != cudaSuccess ? e : cudaGetLastError();
 }

@@ -6,8 +6,7 @@
 // microsecond, for weights of any shape.  A warp owns 16 weight rows and a
 // share of K and loads its weights straight into registers, 16 bytes per lane
 // and sixteen loads deep (eight with two token tiles); no shared memory, no
-// barrier in the loop.  The lanes'
-// 8 consecutive columns are fed to mma.m16n8k16 in place: the MMA sums over k in
+// barrier in the loop.  The lanes' 8 consecutive columns are fed to mma.m16n8k16 in place: the MMA sums over k in
 // any order as long as both operands agree, so lane t of a quad supplies its
 // columns 0..3 and 4..7 as the k positions that the fragment layout gives it,
 // and x, loaded the same way, does too.  (Warp MMAs are far from the tensor
@@ -52,6 +51,10 @@ __device__ __forceinline__ uint4 ldg_stream(const void *p) {
   return v;
 }
 
+// x is the previous kernel's output, which it may still write while this kernel is
+// resident: an ordinary load, not one of read-only data.
+__device__ __forceinline__ uint4 load_x(const uint16_t *p) { return *reinterpret_cast<const uint4 *>(p); }
+
 __device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 template <bool BF16>
@@ -76,13 +79,14 @@ __device__ __forceinline__ uint4 load_tail(const uint16_t *row, uint32_t c, uint
   uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (uint32_t i = 0; i < 8; ++i)
-    if (c + i < cols) w[i / 2u] |= (uint32_t)__ldg(row + c + i) << (16u * (i % 2u));
+    if (c + i < cols) w[i / 2u] |= (uint32_t)row[c + i] << (16u * (i % 2u));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // NT: token tiles of 8.  The cluster's CTAs share 16 weight rows.
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(kMaxWarps * 32, 2) k_linear_narrow(const LinearArgs a, const uint32_t splits, const uint32_t ahead) {
+__global__ void __launch_bounds__(kMaxWarps * 32, 2)
+    k_linear_narrow(const LinearArgs a, const uint32_t splits, const uint32_t ahead) {
   namespace cg = cooperative_groups;
   constexpr uint32_t kDeep = Depth<NT>::value;
   __shared__ float part[kMaxWarps][8 * NT][kRows + 1];
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) k_linear_narrow(const Linea
       for (uint32_t j = 0; j < kDeep; ++j)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          xv[j][n] = token[n] ? __ldg(reinterpret_cast<const uint4 *>(xr[n] + c0 + j * kChunk)) : make_uint4(0u, 0u, 0u, 0u);
+          xv[j][n] = token[n] ? load_x(xr[n] + c0 + j * kChunk) : make_uint4(0u, 0u, 0u, 0u);
     } else {
 #pragma unroll
       for (uint32_t j = 0; j < kDeep; ++j) {
@@ -150,7 +154,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) k_linear_narrow(const Linea
 #pragma unroll
         for (int n = 0; n < NT; ++n)
           xv[j][n] = !token[n] ? make_uint4(0u, 0u, 0u, 0u)
-                     : in      ? __ldg(reinterpret_cast<const uint4 *>(xr[n] + c))
+                     : in      ? load_x(xr[n] + c)
                                : load_tail(xr[n], c, a.cols);
       }
     }

@@ -992,7 +992,8 @@ int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const
   if (!rt) return PW_ERR_ARGUMENT;
   if (!norm || !norm->weight) return fail(rt, PW_ERR_ARGUMENT, "norm descriptor is null");
   if (norm->weight_dtype > PW_NORM_F16) return fail(rt, PW_ERR_ARGUMENT, "unknown norm weight_dtype");
-  if (!std::isfinite(norm->epsilon) || norm->epsilon <= 0.0f) return fail(rt, PW_ERR_ARGUMENT, "invalid RMSNorm epsilon");
+  if (!std::isfinite(norm->epsilon) || norm->epsilon <= 0.0f)
+    return fail(rt, PW_ERR_ARGUMENT, "invalid RMSNorm epsilon");
   // below that, f32 squares that still matter next to it would underflow
   if (norm->epsilon < 1e-30f) return fail(rt, PW_ERR_ARGUMENT, "RMSNorm epsilon below 1e-30");
   if (reinterpret_cast<uintptr_t>(norm->weight) % (norm->weight_dtype == PW_NORM_F32 ? 4u : 2u))
@@ -1003,7 +1004,8 @@ int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const
   if (rows > (1u << 30)) return fail(rt, PW_ERR_UNSUPPORTED, "too many rows");
   if (!codes != !scales) return fail(rt, PW_ERR_ARGUMENT, "codes and scales go together");
   if (!y && !codes) return fail(rt, PW_ERR_ARGUMENT, "nothing asked for: neither y nor codes");
-  if (reinterpret_cast<uintptr_t>(scales) % 4u) return fail(rt, PW_ERR_ARGUMENT, "scales are not aligned to their elements");
+  if (reinterpret_cast<uintptr_t>(scales) % 4u)
+    return fail(rt, PW_ERR_ARGUMENT, "scales are not aligned to their elements");
   int s;
   pw_rows xr{}, rr{}, sr{}, yr{};
   if ((s = check_rows(rt, "x", x, rows, H, xr)) != PW_OK) return s;
@@ -1182,11 +1184,13 @@ int pw_fp8_linear_codes(pw_runtime *rt, const pw_fp8_tensor *w, uint32_t layout,
   int s;
   if ((s = check_projection(rt, w, layout)) != PW_OK) return s;
   if (width > (1u << 30)) return fail(rt, PW_ERR_UNSUPPORTED, "too many rows");
-  if (reinterpret_cast<uintptr_t>(scales) % 4u) return fail(rt, PW_ERR_ARGUMENT, "scales are not aligned to their elements");
+  if (reinterpret_cast<uintptr_t>(scales) % 4u)
+    return fail(rt, PW_ERR_ARGUMENT, "scales are not aligned to their elements");
   const bool host = (mem & PW_MEM_HOST) != 0;
   if ((!host && reinterpret_cast<uintptr_t>(codes) % 16u) || reinterpret_cast<uintptr_t>(w->weight) % 16u)
     return fail(rt, PW_ERR_UNSUPPORTED, "activation codes and weight must start at a 16-byte boundary");
-  if (reinterpret_cast<uintptr_t>(w->scale) % 4u) return fail(rt, PW_ERR_ARGUMENT, "weight scales are not aligned to their elements");
+  if (reinterpret_cast<uintptr_t>(w->scale) % 4u)
+    return fail(rt, PW_ERR_ARGUMENT, "weight scales are not aligned to their elements");
   const uint32_t K = w->cols, N = w->rows;
   pw_rows rr{}, yr{};
   EpilogueArgs e{};

@@ -556,3 +556,162 @@ def test_columns_of_one_buffer_are_not_overlapping(rt):
     want = rt.linear(x, w, residual=buf[:, :32].clone()).output
     rt.linear(x, w, residual=buf[:, :32], out=buf[:, 40:72])
     assert torch.equal(buf[:, 40:72], want)
+
+
+# ------------------------------------------------------------------ streams, graphs, neighbours
+class Layer:
+    """Buffers of one decoder-like layer that a call chain runs over again and again, in place."""
+
+    def __init__(self, width, seed):
+        self.h, self.x = randn((width, 512), seed, torch.bfloat16, 2.0), randn((width, 1024), seed + 1, torch.bfloat16)
+        self.wo = randn((512, 1024), seed + 2, torch.bfloat16, 1 / 32)
+        self.up = randn((768, 512), seed + 3, torch.bfloat16, 1 / 23)
+        self.down = randn((512, 768), seed + 4, torch.bfloat16, 1 / 64)
+        self.norm = randn((512,), seed + 5, torch.bfloat16, 0.1) + 1
+        _, self.b = fp8_case(1, 512, 512, seed + 6)
+
+    def run(self, rt, wait):
+        """Each call takes what the one before it wrote; all over h but the last."""
+        def step(r):
+            if wait:
+                torch.cuda.synchronize()
+            return r
+        for _ in range(3):
+            step(rt.linear(self.x, self.wo, residual=self.h, out=self.h, asynchronous=True))
+            n = step(rt.add_rms_norm(self.h, self.norm, asynchronous=True))
+            m = step(rt.linear(n.y, self.up, activation="silu", asynchronous=True))
+            d = step(rt.linear(m.output, self.down, asynchronous=True))
+            n = step(rt.add_rms_norm(d.output, self.norm, residual=self.h, in_place=True, want_codes=True, asynchronous=True))
+            out = step(rt.fp8_linear_codes(n.codes, n.scales, self.b, residual=self.h, out=self.h, asynchronous=True))
+        return out.output
+
+
+@pytest.mark.parametrize("width", [1, 12, 40, 100, 300])
+def test_two_runtimes_on_two_streams_at_once(width):
+    from mimo_prismwing_b200.runtime import WideMoeRuntime
+    layers = [Layer(width, 200), Layer(width, 210)]
+    rts = [WideMoeRuntime.compile_with_fused_gate_up(0) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    try:
+        want, start = [], [layer.h.clone() for layer in layers]
+        torch.cuda.synchronize()
+        for rt, s, layer in zip(rts, streams, layers):
+            rt.set_stream(s)
+            with torch.cuda.stream(s):
+                want.append(layer.run(rt, True).clone())
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for layer, h in zip(layers, start):
+                layer.h.copy_(h)
+            torch.cuda.synchronize()
+            for rt, s, layer in zip(rts, streams, layers):
+                with torch.cuda.stream(s):
+                    layer.run(rt, False)
+            torch.cuda.synchronize()
+            for layer, w in zip(layers, want):
+                assert torch.equal(layer.h, w)
+        # both captured, replayed at once; inputs in place, so each replay starts over
+        graphs = []
+        for rt, s, layer in zip(rts, streams, layers):
+            with torch.cuda.stream(s):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s):
+                    layer.run(rt, False)
+                graphs.append(g)
+        for _ in range(3):
+            for layer, h in zip(layers, start):
+                layer.h.copy_(h)
+            torch.cuda.synchronize()
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+            torch.cuda.synchronize()
+            for layer, w in zip(layers, want):
+                assert torch.equal(layer.h, w)
+        assert all(rt.error_flags() == 0 for rt in rts)
+    finally:
+        torch.cuda.synchronize()
+        for rt in rts:
+            rt.close()
+
+
+@pytest.mark.parametrize("width", [1, 12, 40, 100, 300])
+def test_first_call_of_a_runtime_may_be_captured(width):
+    from mimo_prismwing_b200.runtime import WideMoeRuntime
+    layer = Layer(width, 220)
+    start = layer.h.clone()
+    rt, s = WideMoeRuntime.compile_with_fused_gate_up(0), torch.cuda.Stream()
+    try:
+        rt.set_stream(s)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                layer.run(rt, False)
+            g.replay()
+            s.synchronize()
+            got = layer.h.clone()
+            layer.h.copy_(start)
+            layer.run(rt, False)
+            s.synchronize()
+        assert torch.equal(layer.h, got) and not torch.equal(got, start)
+    finally:
+        torch.cuda.synchronize()
+        rt.close()
+
+
+@pytest.mark.parametrize("width", [1, 12, 40, 100, 300])
+def test_linear_leaves_what_is_not_its_own(rt, width):
+    # NaN between the rows of x and the weight is not read into a sum, and what
+    # lies between and behind the output's rows stays
+    nan, guard = float("nan"), 7.0
+    x, xb = wide(randn((width, 392), 230, torch.bfloat16), 8, nan)
+    w, wb = wide(randn((200, 392), 231, torch.bfloat16, 0.05), 24, nan)
+    want = rt.linear(x.contiguous(), w.contiguous()).output
+    buf = torch.full((width + 2, 200 + 9), guard, dtype=torch.bfloat16, device="cuda")
+    rt.linear(x, w, out=buf[1:-1, 3:203])
+    assert torch.equal(buf[1:-1, 3:203], want)
+    buf[1:-1, 3:203] = guard
+    assert (buf == guard).all()
+    assert torch.isnan(xb[:, 392:]).all() and torch.isnan(wb[:, 392:]).all()
+
+
+@pytest.mark.parametrize("width", [1, 12, 40, 100, 300])
+def test_fp8_leaves_what_is_not_its_own(rt, width):
+    x, b = fp8_case(width, 384, 512, 232)
+    codes, scales = rt.quantize(x)
+    want = rt.fp8_linear_codes(codes, scales, b).output
+    # the rows behind the last token hold NaN codes and scales
+    more = torch.full((width + 130, 512), 0x7F, dtype=torch.uint8, device="cuda")
+    some = torch.full((width + 130, 4), float("nan"), device="cuda")
+    more[:width], some[:width] = codes, scales
+    buf = torch.full((width + 2, 384 + 9), 7.0, device="cuda")
+    rt.fp8_linear_codes(more[:width], some[:width], b, out=buf[1:-1, 3:387])
+    assert torch.equal(buf[1:-1, 3:387], want)
+    buf[1:-1, 3:387] = 7.0
+    assert (buf == 7.0).all()
+
+
+@pytest.mark.parametrize("rows,hidden", [(1, 512), (5, 513), (3000, 512), (3000, 520)])
+def test_norm_over_its_input_and_beside_its_neighbours(rt, rows, hidden):
+    # through the C call: y may be x itself
+    from mimo_prismwing_b200.runtime import Norm, Rows, MEM_DEVICE
+    w = randn((hidden,), 233) + 1
+    x = randn((rows, hidden), 234, torch.bfloat16, 3.0)
+    want = rt.add_rms_norm(x, w, 1e-5, want_codes=True)
+    buf = torch.full((rows + 2, hidden + 16), 7.0, dtype=torch.bfloat16, device="cuda")
+    v = buf[1:-1, 8:8 + hidden]
+    v.copy_(x)
+    codes = torch.full((rows + 1, hidden), 9, dtype=torch.uint8, device="cuda")
+    groups = -(-hidden // 128)
+    scales = torch.full((rows + 1, groups), 9.0, device="cuda")
+    torch.cuda.synchronize()
+    at = Rows(v.data_ptr(), v.stride(0), 1, 0)
+    norm = Norm(w.data_ptr(), hidden, 0, 1e-5)
+    assert rt._L.pw_add_rms_norm(rt._rt, ctypes.addressof(norm), ctypes.addressof(at), None, rows, None,
+                                 ctypes.addressof(at), codes.data_ptr(), scales.data_ptr(), MEM_DEVICE, None) == 0
+    assert torch.equal(v, want.y)
+    assert torch.equal(codes[:rows], want.codes) and torch.equal(scales[:rows], want.scales)
+    assert (codes[rows] == 9).all() and (scales[rows] == 9).all()
+    v.fill_(7.0)
+    assert (buf == 7.0).all()
