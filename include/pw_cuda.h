@@ -337,7 +337,8 @@ int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const
  * NULL.  A non-finite output is PW_ERR_NONFINITE (PW_FLAG_NONFINITE_ROUND).
  * A token's result does not depend on the other tokens' values, and is the same
  * in every call of the same sizes; other sizes may add the products in another
- * order.  Only calls that convert or copy x use the runtime's scratch. */
+ * order.  A captured call that converts or copies x allocates the copy in the
+ * graph; no other captured call uses memory besides its arguments. */
 int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t width, const pw_epilogue *ep,
               const pw_rows *y, uint32_t mem, pw_stats *stats);
 

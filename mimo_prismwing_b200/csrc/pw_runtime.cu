@@ -948,6 +948,23 @@ cudaError_t copy_rows(const pw_rows &to, const pw_rows &from, uint32_t rows, uin
   return cudaMemcpy2DAsync(to.data, to.stride * z, from.data, from.stride * z, len * z, rows, kind, stream);
 }
 
+// Memory of a captured call: allocated and freed by the graph itself, so that no
+// other graph shares it and no later call moves it, as the runtime's scratch would.
+struct GraphMemory {
+  void *at = nullptr;
+  cudaStream_t stream = nullptr;
+  cudaError_t take(size_t bytes, cudaStream_t s) {
+    stream = s;
+    return cudaMallocAsync(&at, bytes, s);
+  }
+  cudaError_t give() {
+    void *p = at;
+    at = nullptr;
+    return p ? cudaFreeAsync(p, stream) : cudaSuccess;
+  }
+  ~GraphMemory() { give(); }
+};
+
 // Checks an epilogue and its output rows and turns them into kernel arguments;
 // with the residual's and y's caller rows in `res` and `out`.
 int check_epilogue(pw_runtime *rt, const pw_epilogue *ep, const pw_rows *y, uint32_t width, uint32_t cols,
@@ -1124,6 +1141,12 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
   CK(dev.enter(rt->device));
   Call call{rt, mem, stats, 0};
   if ((s = call.begin()) != PW_OK) return s;
+  // TMA reads rows that start at 16-byte boundaries, of the weight's type
+  const bool convert = xr.dtype != w->dtype || (!call.host() && (reinterpret_cast<uintptr_t>(xr.data) % 16u ||
+                                                                 xr.stride % 8u || xr.stride >= ((uint64_t)1 << 36)));
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (convert && !call.host()) CK(cudaStreamIsCapturing(rt->stream, &capture));
+  GraphMemory graph;
   Arena ar;
   for (int pass = 0; pass < 2; ++pass) {
     if (pass == 1) {
@@ -1136,15 +1159,17 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
       if (rr.data) dr = device_rows(ar, rr, width, N);
       dy = device_rows(ar, yr, width, N);
     }
-    // TMA reads rows that start at 16-byte boundaries, of the weight's type
-    const bool convert = xr.dtype != w->dtype || (!call.host() && (reinterpret_cast<uintptr_t>(xr.data) % 16u ||
-                                                                   xr.stride % 8u || xr.stride >= ((uint64_t)1 << 36)));
     pw_rows cx = dx;
     if (convert) {
       cx.dtype = w->dtype;
-      cx = device_rows(ar, cx, width, K);
+      Arena none;
+      cx = device_rows(capture == cudaStreamCaptureStatusNone ? ar : none, cx, width, K);
     }
     if (pass == 0) continue;
+    if (convert && capture != cudaStreamCaptureStatusNone) {
+      CK(graph.take((size_t)width * cx.stride * 2u, rt->stream));
+      cx.data = graph.at;
+    }
     if (call.host()) {
       CK(copy_rows(dx, xr, width, K, cudaMemcpyHostToDevice, rt->stream));
       if (rr.data) CK(copy_rows(dr, rr, width, N, cudaMemcpyHostToDevice, rt->stream));
@@ -1170,6 +1195,7 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
       PdlScope pdl(!rt->profiling);
       CK(launch_linear(a, rt->num_sms, rt->stream));
     }
+    CK(graph.give());
     if (call.host()) CK(copy_rows(yr, dy, width, N, cudaMemcpyDeviceToHost, rt->stream));
   }
   return call.finish((uint64_t)N * K * 2u);

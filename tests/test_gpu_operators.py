@@ -715,3 +715,42 @@ def test_norm_over_its_input_and_beside_its_neighbours(rt, rows, hidden):
     assert (codes[rows] == 9).all() and (scales[rows] == 9).all()
     v.fill_(7.0)
     assert (buf == 7.0).all()
+
+
+@pytest.mark.parametrize("width", [1, 40, 300])
+def test_graphs_that_convert_x_share_nothing(width):
+    # two graphs of one runtime over float32 and unaligned rows, replayed at once
+    # after a larger call has moved the runtime's own memory
+    from mimo_prismwing_b200.runtime import WideMoeRuntime
+    rt, streams = WideMoeRuntime.compile_with_fused_gate_up(0), [torch.cuda.Stream() for _ in range(2)]
+    w = [randn((512, 1024), 240 + i, torch.bfloat16, 0.03) for i in range(2)]
+    x = [randn((width, 1024), 242 + i, torch.bfloat16).float() for i in range(2)]
+    odd = [wide(t.bfloat16(), 3)[0] for t in x]
+    try:
+        outs, graphs = [], []
+        torch.cuda.synchronize()
+        for s, wi, xi, oi in zip(streams, w, x, odd):
+            rt.set_stream(s)
+            with torch.cuda.stream(s):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s):
+                    outs.append([rt.linear(t, wi, out_dtype=torch.bfloat16, asynchronous=True).output
+                                 for t in (xi, oi, xi, oi)])
+                graphs.append(g)
+        rt.set_stream(torch.cuda.current_stream())
+        rt.linear(randn((3000, 4096), 244), randn((64, 4096), 245, torch.bfloat16))
+        want = [rt.linear(xi.bfloat16(), wi).output for wi, xi in zip(w, x)]
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+            torch.cuda.synchronize()
+            for got, ref in zip(outs, want):
+                for y in got:
+                    assert torch.equal(y, ref)
+                    y.zero_()
+            torch.cuda.synchronize()
+    finally:
+        torch.cuda.synchronize()
+        rt.close()
