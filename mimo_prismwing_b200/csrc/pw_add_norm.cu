@@ -24,6 +24,7 @@ namespace pw {
 namespace addnorm {
 
 constexpr uint32_t kMaxThreads = 512;
+constexpr uint32_t kSlimThreads = 128;
 constexpr uint32_t kMaxHidden = 16384;
 
 // How a thread's step of 8 columns is accessed: element by element, as 16-byte
@@ -193,8 +194,9 @@ __device__ __forceinline__ void fetch_row(const AddNormArgs &a, uint8_t *ring, u
 
 // STEPS: steps of 8 columns per thread (hidden <= 8 * STEPS * blockDim.x).
 // stages: ring slots, or 0 to load rows straight into registers.
-template <typename T, Access VEC, int STEPS>
-__global__ void __launch_bounds__(kMaxThreads, STEPS == 1 ? 3 : STEPS == 2 ? 2 : 1)
+// SLIM: registers for a fifth CTA of four warps per SM.
+template <typename T, Access VEC, int STEPS, bool SLIM>
+__global__ void __launch_bounds__(SLIM ? kSlimThreads : kMaxThreads, SLIM ? 5 : STEPS == 1 ? 3 : STEPS == 2 ? 2 : 1)
     k_add_norm(const AddNormArgs a, const uint32_t stages) {
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float part[2][kMaxThreads / 32];
@@ -426,9 +428,9 @@ uint32_t resident(uint32_t threads) {
   return (uint32_t)n;
 }
 
-template <typename T, Access VEC, int STEPS>
+template <typename T, Access VEC, int STEPS, bool SLIM>
 cudaError_t launch_one(const AddNormArgs &a, uint32_t threads, int num_sms, cudaStream_t stream) {
-  const uint32_t per_sm = resident<k_add_norm<T, VEC, STEPS>>(threads);
+  const uint32_t per_sm = resident<k_add_norm<T, VEC, STEPS, SLIM>>(threads);
   uint32_t stages = 0;
   // The ring pays when CTAs run several rows (without it the first and last case
   // below took 21.5 and 204 us).  Slots share what the resident CTAs have of shared memory.
@@ -440,17 +442,29 @@ cudaError_t launch_one(const AddNormArgs &a, uint32_t threads, int num_sms, cuda
   const uint32_t most = (uint32_t)num_sms * per_sm;
   const uint32_t grid = a.rows < most ? a.rows : most;
   if (stages) {
-    cudaError_t e = allow_smem<k_add_norm<T, VEC, STEPS>>(kRingBytes);
+    cudaError_t e = allow_smem<k_add_norm<T, VEC, STEPS, SLIM>>(kRingBytes);
     if (e != cudaSuccess) return e;
   }
-  return launch_kernel(k_add_norm<T, VEC, STEPS>, dim3(grid), dim3(threads), stages * row_bytes, stream, a, stages);
+  return launch_kernel(k_add_norm<T, VEC, STEPS, SLIM>, dim3(grid), dim3(threads), stages * row_bytes, stream, a, stages);
 }
 
 template <typename T, Access VEC>
 cudaError_t launch_shape(const AddNormArgs &a, uint32_t steps, uint32_t threads, int num_sms, cudaStream_t stream) {
-  if (steps == 1u) return launch_one<T, VEC, 1>(a, threads, num_sms, stream);
-  if (steps == 2u) return launch_one<T, VEC, 2>(a, threads, num_sms, stream);
-  return launch_one<T, VEC, 4>(a, threads, num_sms, stream);
+  if (steps == 1u) return launch_one<T, VEC, 1, false>(a, threads, num_sms, stream);
+  if (steps == 2u) return launch_one<T, VEC, 2, false>(a, threads, num_sms, stream);
+  // Fewer registers make more CTAs resident, and a turn of each slower: worth it when
+  // the rows then take fewer turns (bf16 with residual and codes, usual / slim: 2048 x
+  // 4096, 4 / 3 turns, 15.8 / 14.4 us; 16384 x 1024, 7 / 6 turns, 23.9 / 23.0 us; 2048 x
+  // 2048, 2 turns both, 7.0 / 7.7 us; f32 rows leave slim CTAs no ring: 35.7 / 39.2 us).
+  if constexpr (VEC != kElements && sizeof(T) == 2) {
+    if (threads <= kSlimThreads) {
+      const uint32_t usual = resident<k_add_norm<T, VEC, 4, false>>(threads) * (uint32_t)num_sms;
+      const uint32_t slim = resident<k_add_norm<T, VEC, 4, true>>(threads) * (uint32_t)num_sms;
+      if ((a.rows + slim - 1u) / slim < (a.rows + usual - 1u) / usual)
+        return launch_one<T, VEC, 4, true>(a, threads, num_sms, stream);
+    }
+  }
+  return launch_one<T, VEC, 4, false>(a, threads, num_sms, stream);
 }
 
 template <typename T, Access VEC>

@@ -104,7 +104,8 @@ def test_norm_matches_its_definition(rt, rows, hidden, dtype):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("rows,hidden,residual", [(4001, 512, True), (2500, 4096, True), (2500, 4096, False),
-                                                  (700, 8192, True), (400, 16384, False), (300, 16384, True)])
+                                                  (700, 8192, True), (400, 16384, False), (300, 16384, True),
+                                                  (2500, 1000, True), (2500, 1024, False)])
 def test_norm_over_many_rows(rt, rows, hidden, residual, dtype):
     # several rows per CTA, in place over the stream
     t = TYPES[dtype]
