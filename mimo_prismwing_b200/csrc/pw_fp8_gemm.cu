@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         w1 = __ldg(a.ws + (uint64_t)s1 * kblocks + lane);
       }
     };
-    const uint32_t tempty_lead = map_rank(smem_addr(sh.tempty), lead);  // the leading CTA's
+    const uint32_t tempty_lead = map_rank(smem_addr(sh.tempty), cta & ~(CTAS - 1u));  // the leading CTA's
     const bool quad_r = quad_access(a.ep.residual, a.ep.residual_stride, a.ep.residual_dtype);
     const bool quad_y = quad_access(a.ep.y, a.ep.y_stride, a.ep.y_dtype);
     uint32_t acc_slot = 0, aphase = 0, ti = 0;
@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       tc::cp_async_wait_all();
       named_bar_sync(2u + quarter, 64u);  // this tile's scales are here, the other buffer is free
       float *xsb = sh.xs + ((ti & 1u) * 4u + quarter) * (kMaxBlocks * 32u);
+      const uint32_t xs_at = smem_addr(xsb + lane);
       if (u + u_step < total) xs_fetch(u + u_step, (ti & 1u) ^ 1u);
       const float wc0 = wn0, wc1 = wn1;
       if (u + u_step < total) ws_load(u + u_step, wn0, wn1);
@@ -359,61 +360,66 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
 #pragma unroll
       for (uint32_t i = 0; i < C::COLS; ++i) acc[i] = 0.0f;
       if (active) {
-        // A chunk of 32 columns loads while the previous one is promoted, across
-        // blocks too; the accumulator goes back to the MMA once its last chunk is
-        // in registers.  The next block's scales are read a block ahead.
+        // A chunk of 32 columns loads while the previous one is promoted; the
+        // accumulator goes back to the MMA once its last chunk is in registers.  A warp
+        // issues in order, so what takes long to come back is asked for early: the next
+        // block's scales at the block's start (multiplied at its end), the next
+        // accumulator's barrier half a chunk before it is needed.
         float v[2][32];
-        auto scales = [&](uint32_t kb, float &s0, float &s1) {
-          const float x = xsb[kb * 32u + lane];
-          s0 = __fmul_rn(__shfl_sync(0xffffffffu, wc0, kb), x);
-          s1 = C::COLS > 64u ? __fmul_rn(__shfl_sync(0xffffffffu, wc1, kb), x) : s0;
+        uint32_t x1, p0, p1;  // the next block's scales: the token's, the weight's
+        auto ask = [&](uint32_t kb) {
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x1) : "r"(xs_at + kb * 128u));
+          p0 = __shfl_sync(0xffffffffu, __float_as_uint(wc0), kb);
+          if (CH > 2u) p1 = __shfl_sync(0xffffffffu, __float_as_uint(wc1), kb);
         };
         float s0, s1;
-        scales(kb0, s0, s1);
-        bool ok = __all_sync(0xffffffffu, bounded_wait(sh.abort, &sh.tfull[acc_slot], aphase, a.flags));
+        auto answer = [&]() {
+          s0 = __fmul_rn(__uint_as_float(p0), __uint_as_float(x1));
+          s1 = CH > 2u ? __fmul_rn(__uint_as_float(p1), __uint_as_float(x1)) : s0;
+        };
+        ask(kb0);
+        bounded_wait(sh.abort, &sh.tfull[acc_slot], aphase, a.flags);
+        __syncwarp();
         tc_fence_after();
         tc::tmem_ld32(cols + acc_slot * BN, v[0]);
+        answer();
         tc::tmem_wait_ld(v[0]);
 #pragma unroll 1
         for (uint32_t kb = kb0; kb < kb1; ++kb) {
-          if (!ok) s0 = s1 = 0.0f;
           const bool more = kb + 1u < kb1;
-          float n0 = 0.0f, n1 = 0.0f;
 #pragma unroll
           for (uint32_t q = 0; q < CH; ++q) {
             const float s = q < 2u ? s0 : s1;
             float(&now)[32] = v[q & 1u];
             float(&next)[32] = v[(q & 1u) ^ 1u];
-            bool load = true;
-            if (q + 1u < CH) {
+            const bool last = q + 1u == CH;
+            bool ready = true;
+            if (!last) {
               tc::tmem_ld32(cols + acc_slot * BN + 32u * (q + 1u), next);
-              if (q == 0u && more) scales(kb + 1u, n0, n1);
+              if (q == 0u && more) ask(kb + 1u);
             } else {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) {
-                if (PAIR)
-                  arrive_relaxed_remote(tempty_lead + acc_slot * 8u);
-                else
-                  arrive_relaxed(&sh.tempty[acc_slot]);
-              }
+              if (lane == 0) arrive_relaxed_remote(tempty_lead + acc_slot * 8u);
               if (++acc_slot == NACC) {
                 acc_slot = 0;
                 aphase ^= 1u;
               }
-              load = more;
-              if (load) {
-                ok = __all_sync(0xffffffffu, bounded_wait(sh.abort, &sh.tfull[acc_slot], aphase, a.flags));
-                tc_fence_after();
-                tc::tmem_ld32(cols + acc_slot * BN, next);
-              }
+              if (more) ready = look<false, false>(&sh.tfull[acc_slot], aphase);
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) acc[32u * q + i] = __fmaf_rn(now[i], s, acc[32u * q + i]);
-            if (load) tc::tmem_wait_ld(next);
+            for (int i = 0; i < 16; ++i) acc[32u * q + i] = __fmaf_rn(now[i], s, acc[32u * q + i]);
+            if (last && more) {
+              if (!ready) bounded_wait(sh.abort, &sh.tfull[acc_slot], aphase, a.flags);
+              __syncwarp();
+              tc_fence_after();
+              tc::tmem_ld32(cols + acc_slot * BN, next);
+            }
+#pragma unroll
+            for (int i = 16; i < 32; ++i) acc[32u * q + i] = __fmaf_rn(now[i], s, acc[32u * q + i]);
+            if (!last || more) tc::tmem_wait_ld(next);
           }
-          s0 = n0;
-          s1 = n1;
+          answer();
         }
       } else {
         // no tokens or no rows here: keep the accumulators' handshake
@@ -422,12 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
           tc_fence_after();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            if (PAIR)
-              arrive_relaxed_remote(tempty_lead + acc_slot * 8u);
-            else
-              arrive_relaxed(&sh.tempty[acc_slot]);
-          }
+          if (lane == 0) arrive_relaxed_remote(tempty_lead + acc_slot * 8u);
           if (++acc_slot == NACC) {
             acc_slot = 0;
             aphase ^= 1u;
