@@ -27,6 +27,19 @@ __device__ __forceinline__ void mma_commit_pair_elect(uint64_t *bar, uint32_t pa
       "h"((uint16_t)pair_mask)
       : "memory");
 }
+// The same for a kernel whose MMAs one thread issues; without PAIR on this CTA's barrier.
+template <bool PAIR>
+__device__ __forceinline__ void mma_commit(uint64_t *bar, uint32_t pair_mask) {
+  if (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_addr(bar)),
+        "h"((uint16_t)pair_mask)
+        : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
 // A tile load into this CTA's shared memory that completes on the pair's
 // leading CTA's barrier (a shared::cluster address).
 __device__ __forceinline__ void tma_load_pair(void *dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {

@@ -93,14 +93,23 @@ struct Shared {
   volatile int *abort;
 };
 
-__device__ __forceinline__ void mma_f8_pair_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accum)
-      : "memory");
+// For the thread that issues them all.
+template <bool PAIR>
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accum)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accum)
+        : "memory");
 }
 
 __device__ __forceinline__ void tile_of(const Args &A, uint32_t u, uint32_t &row_tile, uint32_t &token_tile) {
@@ -240,7 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         for (uint32_t i = 0; i < NST; ++i)
           if (issued & (1u << i))
             if (!mbar_wait(&sh.full[i], (parity >> i) & 1u)) raise_flag(a.flags, PW_FLAG_WAIT_TIMEOUT);
-    } else if (warp == (uint32_t)kMmaWarp && rank == 0u) {
+    } else if (warp == (uint32_t)kMmaWarp && rank == 0u && elect_one()) {
+      // one thread: an election per instruction costs as much as an MMA takes
       const uint32_t idesc = tc::instr_desc(BN, CTAS * kTileRows);
       const uint64_t ring_desc = smem_desc_sw128(smem_addr(sh.ring));
       uint32_t slot = 0, phase = 0, acc = 0, aphase = 0, pending = 0, pend_parity = 0;
@@ -259,17 +269,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
               const uint64_t ad = ring_desc + ((slot * C::STAGE + j * A.box_tokens * 128u) >> 4);
               const uint64_t bd = ring_desc + ((slot * C::STAGE + C::A_BYTES + j * 128u * 128u) >> 4);
 #pragma unroll
-              for (uint32_t s = 0; s < 4; ++s) {
-                if (PAIR)
-                  mma_f8_pair_elect(d, ad + 2u * s, bd + 2u * s, idesc, s ? 1u : 0u);
-                else
-                  tc::mma_f8_elect(d, ad + 2u * s, bd + 2u * s, idesc, s ? 1u : 0u);
-              }
+              for (uint32_t s = 0; s < 4; ++s) mma_f8<PAIR>(d, ad + 2u * s, bd + 2u * s, idesc, s ? 1u : 0u);
             }
-            if (PAIR)
-              mma_commit_pair_elect(&sh.tfull[acc], 3u << lead);
-            else
-              tc::mma_commit_elect(&sh.tfull[acc]);
+            mma_commit<PAIR>(&sh.tfull[acc], 3u << lead);
             pending |= 1u << acc;
             pend_parity = (pend_parity & ~(1u << acc)) | (aphase << acc);
             if (++acc == NACC) {
@@ -277,10 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
               aphase ^= 1u;
             }
           }
-          if (PAIR)
-            mma_commit_pair_elect(&sh.empty[slot], 3u << lead);
-          else
-            tc::mma_commit_elect(&sh.empty[slot]);
+          mma_commit<PAIR>(&sh.empty[slot], 3u << lead);
           if (++slot == NST) {
             slot = 0;
             phase ^= 1u;
@@ -292,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         if (pending & (1u << i))
           if (!mbar_wait(&sh.tfull[i], (pend_parity >> i) & 1u)) raise_flag(a.flags, PW_FLAG_WAIT_TIMEOUT);
     }
+    __syncwarp();
     if (splits > 1u) {
       // the epilogue's two cluster barriers count every thread
       __syncwarp();
