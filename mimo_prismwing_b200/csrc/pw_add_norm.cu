@@ -113,13 +113,6 @@ __device__ __forceinline__ void add_words(uint4 &a, uint4 b) {
   for (int i = 0; i < 4; ++i) p[i] = __hadd2(p[i], q[i]);
 }
 
-// max(|a|, |b|, |c|), a NaN if any is one.
-__device__ __forceinline__ float max_abs(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
-  return d;
-}
-
 // The group's quotient as Fp8GroupScale::quotient; the conversion to e4m3 saturates.
 __device__ __forceinline__ float code_quotient(const Fp8GroupScale &g, float v) {
   const float q0 = __fmul_rn(v, g.rcp);

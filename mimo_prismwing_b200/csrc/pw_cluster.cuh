@@ -82,6 +82,19 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
+// A box from shared memory to global memory, and the end of its reading for all but
+// the last N boxes that this thread sent.
+__device__ __forceinline__ void tma_store(const CUtensorMap *map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+               "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+
 // One look at a barrier's phase; SLEEP: waits in hardware for up to 100 us, woken
 // by the phase's completion.  PAIR: the pair's other CTA arrives on the barrier too.
 template <bool PAIR, bool SLEEP>

@@ -132,6 +132,27 @@ __device__ __forceinline__ void activate_all(float (&v)[N], uint32_t act) {
   }
 }
 
+// max(|a|, |b|, |c|), a NaN if any is one.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return d;
+}
+
+// 8 values in a 16-byte word of a 16-bit type.
+__device__ __forceinline__ uint4 pack8(const float *v, uint32_t dtype) {
+  if (dtype == PW_DTYPE_BF16)
+    return make_uint4(pack_bf16x2_rn(v[0], v[1]), pack_bf16x2_rn(v[2], v[3]), pack_bf16x2_rn(v[4], v[5]),
+                      pack_bf16x2_rn(v[6], v[7]));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t *>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Whether four consecutive elements from any column c, c % 4 == 0, of these rows can
 // be accessed at once.
 __device__ __forceinline__ bool quad_access(const void *p, uint64_t stride, uint32_t dtype) {

@@ -66,10 +66,13 @@ struct Cfg {
   static constexpr uint32_t A_BYTES = KBS * kTileRows * 128u;
   static constexpr uint32_t B_BYTES = KBS * 128u * 128u;  // this CTA's 128 weight rows
   static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
-  static constexpr uint32_t NST = PAIR ? 6u : 3u;
+  static constexpr uint32_t NST = PAIR ? 5u : 3u;
   static constexpr uint32_t NACC = PAIR ? 2u : 4u;
   static constexpr uint32_t COLS = BN / 2u;  // a thread's columns: two warps per lane quarter
-  static constexpr uint32_t XS = NST * STAGE;  // token scales [2 tiles][4 quarters][32 blocks][32 tokens] f32
+  // 2 KB output boxes per epilogue warp; one CTA's one is in the scale buffer
+  static constexpr uint32_t BOXES = PAIR ? 2u : 1u;
+  static constexpr uint32_t STG = NST * STAGE;
+  static constexpr uint32_t XS = STG + (PAIR ? kEpiWarps * BOXES * 2048u : 0u);  // token scales [2 tiles][4 quarters][32 blocks][32 tokens] f32
   static constexpr uint32_t BARS = XS + 2u * 4u * kMaxBlocks * 32u * 4u;
   static constexpr uint32_t MISC = BARS + (2u * NST + 2u * NACC) * 8u;
   static constexpr uint32_t SMEM = MISC + 16u + 1024u;  // + alignment slack
@@ -80,7 +83,8 @@ struct Cfg {
 
 struct Args {
   Fp8CodesArgs a;
-  CUtensorMap wmap, xmap;
+  CUtensorMap wmap, xmap, ymap;
+  bool tma_y;  // outputs by way of ymap: no residual, rows at 16-byte boundaries
   uint32_t row_tiles, token_tiles, stages, splits;
   uint32_t box_tokens;  // token rows that a stage loads
 };
@@ -349,6 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       const uint32_t c_base = rt * BN + col0;  // the warp's first output column
       const bool active = rows_here != 0u && c_base < a.rows;
       tc::cp_async_wait_all();
+      if (!PAIR && lane == 0) tma_store_wait_read<0>();  // the last tile's outputs have left the other buffer
       named_bar_sync(2u + quarter, 64u);  // this tile's scales are here, the other buffer is free
       float *xsb = sh.xs + ((ti & 1u) * 4u + quarter) * (kMaxBlocks * 32u);
       const uint32_t xs_at = smem_addr(xsb + lane);
@@ -482,6 +487,76 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
             ok = finish_quads(a.ep, now, v, cur_bias, cur, quad_r, quad_y) && ok;
           }
         if (!ok) raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
+      } else if (A.tma_y) {
+        // Each thread packs its token's next 32 columns into a 64-byte row of a box
+        // (two boxes of f32; 16-byte chunk i at position i ^ ((token >> 1) & 3)), which
+        // leaves by TMA while the next is made.  The loop is rolled (the sums move down
+        // 32 registers per turn): unrolled, its code left the instruction cache and a
+        // tile's epilogue took as long as its products.
+        // lane l loads the bias of the warp's columns 4 l .. 4 l + 3
+        float4 biasc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (active && 4u * lane < C::COLS) biasc = bias4(a.ep, c_base + 4u * lane);
+        if (!PAIR) named_bar_sync(2u + quarter, 64u);  // both warps are done with the scales
+        if (active) {
+          const uint32_t stg = PAIR ? smem_addr(smem + C::STG + (warp - kEpiWarp0) * (C::BOXES * 2048u))
+                                    : smem_addr(xsb) + half * 2048u;
+          uint32_t box = 0;
+          float most = 0.0f;
+          auto put = [&](uint32_t col, const uint4(&w)[4]) {
+            if (lane == 0) tma_store_wait_read<C::BOXES - 1u>();
+            __syncwarp();
+            const uint32_t to = stg + box * 2048u;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + lane * 64u +
+                                                                            ((i ^ ((lane >> 1) & 3u)) << 4)),
+                           "r"(w[i].x), "r"(w[i].y), "r"(w[i].z), "r"(w[i].w)
+                           : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tma_store(&A.ymap, (int)col, (int)tok_q, to);
+            if (C::BOXES > 1u) box ^= 1u;
+          };
+#pragma unroll 1
+          for (uint32_t h = 0; h < C::COLS / 32u; ++h) {
+            float v[32];
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) v[i] = acc[i];
+            if (a.ep.bias) {
+#pragma unroll
+              for (uint32_t j = 0; j < 8; ++j) {
+                v[4u * j] += __shfl_sync(0xffffffffu, biasc.x, h * 8u + j);
+                v[4u * j + 1u] += __shfl_sync(0xffffffffu, biasc.y, h * 8u + j);
+                v[4u * j + 2u] += __shfl_sync(0xffffffffu, biasc.z, h * 8u + j);
+                v[4u * j + 3u] += __shfl_sync(0xffffffffu, biasc.w, h * 8u + j);
+              }
+            }
+            activate_all(v, a.ep.act);
+#pragma unroll
+            for (uint32_t i = 0; i < 32; i += 2) most = max_abs(most, v[i], v[i + 1u]);
+            const uint32_t col = c_base + 32u * h;
+            uint4 w[4];
+            if (a.ep.y_dtype == PW_DTYPE_F32) {
+#pragma unroll
+              for (uint32_t b = 0; b < 2; ++b) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                  w[i] = make_uint4(__float_as_uint(v[16u * b + 4u * i]), __float_as_uint(v[16u * b + 4u * i + 1u]),
+                                    __float_as_uint(v[16u * b + 4u * i + 2u]), __float_as_uint(v[16u * b + 4u * i + 3u]));
+                put(col + 16u * b, w);
+              }
+            } else {
+#pragma unroll
+              for (uint32_t i = 0; i < 4; ++i) w[i] = pack8(v + 8u * i, a.ep.y_dtype);
+              put(col, w);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i + 32u < C::COLS; ++i) acc[i] = acc[i + 32u];
+          }
+          // a token past the end (its sums are of no value) is not stored
+          if (tok_q + lane < a.width && __float_as_uint(most) >= overflow_bits(a.ep.y_dtype))
+            raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
+        }
       } else {
         // Outputs through staging rows in this tile's scale buffer, which the
         // quarter no longer needs once both of its warps are past the last block:
@@ -537,6 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
     }
   }
 
+  if (warp >= (uint32_t)kEpiWarp0 && lane == 0) tma_store_wait_read<0>();
   tc_fence_before();
   __syncthreads();
   if (PAIR) {
@@ -592,6 +668,8 @@ cudaError_t launch_one(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream) 
   if (!encode_weight_map(&A.wmap, a.w, a.rows, a.K, qkv ? 64u : 128u, qkv ? 1u : C::KBS) ||
       !encode_weight_map(&A.xmap, a.codes, a.width, a.K, A.box_tokens, C::KBS))
     return cudaErrorInvalidValue;
+  A.tma_y = a.ep.residual == nullptr && reinterpret_cast<uintptr_t>(a.ep.y) % 16u == 0u &&
+            encode_out_map(&A.ymap, a.ep.y, a.width, a.rows, a.ep.y_stride, a.ep.y_dtype, 32u);
   const uint64_t tiles = (uint64_t)A.row_tiles * A.token_tiles, at_once = (uint64_t)num_sms / CTAS;
   if (tiles > 0x7fffffffull / kMaxSplits) return cudaErrorInvalidValue;
   const uint32_t clusters = (uint32_t)(A.splits > 1u ? tiles * A.splits : tiles < at_once ? tiles : at_once);

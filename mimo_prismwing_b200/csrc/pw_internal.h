@@ -278,6 +278,8 @@ cudaError_t launch_convert_rows(const void *x, uint64_t x_stride, uint32_t x_dty
 // cuTensorMapEncodeTiled over 16-bit rows: with k_blocks, the view {64
 // columns, rows, cols / 64} in boxes {64, box_rows, k_blocks}; without, the
 // view {cols, rows, 1} in boxes {64, box_rows, 1}, zero past the last column.
+bool encode_out_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride, uint32_t dtype,
+                    uint32_t box_rows);
 bool encode_rows16_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride,
                        uint32_t dtype, uint32_t box_rows, uint32_t k_blocks);
 

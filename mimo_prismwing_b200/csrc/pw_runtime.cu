@@ -67,6 +67,25 @@ bool encode_act_maps(CUtensorMap (&out)[4], const void *base, uint32_t rows, uin
 }
 
 // 16-bit rows for the linear layer's TMA loads (zero past every end).
+// Output rows as boxes of 64 bytes x box_rows, 64B-swizzled.
+bool encode_out_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride, uint32_t dtype,
+                    uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  const uint32_t z = dtype == PW_DTYPE_F32 ? 4u : 2u;
+  if (!fn || rows == 0 || cols == 0 || stride * z % 16u) return false;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {stride * z};
+  cuuint32_t box[2] = {64u / z, box_rows};
+  cuuint32_t estr[2] = {1u, 1u};
+  return fn(out,
+            dtype == PW_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+            : dtype == PW_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+            2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
 bool encode_rows16_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride,
                        uint32_t dtype, uint32_t box_rows, uint32_t k_blocks) {
   EncodeTiledFn fn = encode_fn();

@@ -691,6 +691,13 @@ def test_fp8_leaves_what_is_not_its_own(rt, width):
     assert torch.equal(buf[1:-1, 3:387], want)
     buf[1:-1, 3:387] = 7.0
     assert (buf == 7.0).all()
+    # rows that start at 16-byte boundaries leave by another way
+    for out, cols in ((torch.float32, 4), (torch.bfloat16, 8), (torch.float16, 16)):
+        buf = torch.full((width + 2, 384 + 32), 7.0, dtype=out, device="cuda")
+        rt.fp8_linear_codes(more[:width], some[:width], b, out=buf[1:-1, cols:cols + 384])
+        assert torch.equal(buf[1:-1, cols:cols + 384], want.to(out))
+        buf[1:-1, cols:cols + 384] = 7.0
+        assert (buf == 7.0).all()
 
 
 @pytest.mark.parametrize("rows,hidden", [(1, 512), (5, 513), (3000, 512), (3000, 520)])
