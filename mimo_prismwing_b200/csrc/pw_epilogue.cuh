@@ -153,6 +153,18 @@ __device__ __forceinline__ uint4 pack8(const float *v, uint32_t dtype) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// v[i] += 8 values of a 16-bit type.
+__device__ __forceinline__ void add8(float *v, uint4 q, uint32_t dtype) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = dtype == PW_DTYPE_BF16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u))
+                                            : __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+    v[2 * i] += f.x;
+    v[2 * i + 1] += f.y;
+  }
+}
+
 // Whether four consecutive elements from any column c, c % 4 == 0, of these rows can
 // be accessed at once.
 __device__ __forceinline__ bool quad_access(const void *p, uint64_t stride, uint32_t dtype) {

@@ -49,42 +49,46 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint32_t kSmemLimit = 227u * 1024u;
 constexpr uint32_t kMaxBlocks = 32;   // K <= 4096
-// Measured cycles (256 or more tokens of 4096 columns, B200 at 1.9 GHz): the one-CTA
-// tile 900 per block and 10000 per wave, a pair's, of four times the products, 1000
-// and 21000.  They meet at 512 tokens of [4096, 4096] (23.4 and 24.8 us); 1024
-// tokens take 44 and 31 us, 203 of [4096, 2048] 11.8 and 16.2 us.
-constexpr TileCost kCostOne{900u, 10000u, 12000u}, kCostPair{1000u, 21000u, 26000u};
+// Measured cycles (B200 at 1.9 GHz): the one-CTA tile 800 per block and 6000 per wave, a
+// pair's, of four times the products, 1150 and 9000; joining K splits costs 13500 and
+// 28000 in place of the latter.  In us, one CTA / pair: 512 x 4096 x 4096 18.0 / 24.4, 768 x
+// 4096 x 4096 33.1 / 26.3, 256 x 13568 x 4096 33.8 / 27.2; unsplit / split one-CTA tiles: 203 x 4096 x
+// 2048 10.1 / 10.8, 64 x 4096 x 4096 15.8 / 11.0.
+constexpr TileCost kCostOne{800u, 6000u, 13500u}, kCostPair{1150u, 9000u, 28000u};
 constexpr uint32_t kTokenGroup = 8;   // token tiles that neighbouring pairs share weights over
 // Register split of PAIR: 256 x 240 + 128 x 24, all of the 384 x 168 at launch.
 constexpr int kRegsLaunch = 168, kRegsEpi = 240, kRegsOther = 24;
 static_assert(kEpiWarps * 32 * kRegsEpi + kEpiWarp0 * 32 * kRegsOther <= kThreads * kRegsLaunch, "register split");
 
-template <bool PAIR>
+// RES: the residual comes into the output boxes by TMA.  It takes more boxes to hide,
+// and the ring gives way (2048 x 16384 x 4096, us with / without a residual: four stages
+// and four boxes 186 / 181, five and two 190+ / 171).
+template <bool PAIR, bool RES>
 struct Cfg {
   static constexpr uint32_t BN = PAIR ? 256u : 128u;    // weight rows of a tile
-  static constexpr uint32_t KBS = PAIR ? 1u : 2u;       // column blocks per stage
-  static constexpr uint32_t A_BYTES = KBS * kTileRows * 128u;
-  static constexpr uint32_t B_BYTES = KBS * 128u * 128u;  // this CTA's 128 weight rows
+  static constexpr uint32_t A_BYTES = kTileRows * 128u;  // a stage is one column block
+  static constexpr uint32_t B_BYTES = 128u * 128u;       // this CTA's 128 weight rows
   static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
-  static constexpr uint32_t NST = PAIR ? 5u : 3u;
+  static constexpr uint32_t NST = RES ? 4u : 5u;
   static constexpr uint32_t NACC = PAIR ? 2u : 4u;
   static constexpr uint32_t COLS = BN / 2u;  // a thread's columns: two warps per lane quarter
-  // 2 KB output boxes per epilogue warp; one CTA's one is in the scale buffer
-  static constexpr uint32_t BOXES = PAIR ? 2u : 1u;
+  static constexpr uint32_t BOXES = RES ? 4u : 2u;  // 2 KB output boxes per epilogue warp
   static constexpr uint32_t STG = NST * STAGE;
-  static constexpr uint32_t XS = STG + (PAIR ? kEpiWarps * BOXES * 2048u : 0u);  // token scales [2 tiles][4 quarters][32 blocks][32 tokens] f32
+  static constexpr uint32_t XS = STG + kEpiWarps * BOXES * 2048u;  // token scales [2 tiles][4 quarters][32 blocks][32 tokens] f32
   static constexpr uint32_t BARS = XS + 2u * 4u * kMaxBlocks * 32u * 4u;
-  static constexpr uint32_t MISC = BARS + (2u * NST + 2u * NACC) * 8u;
+  static constexpr uint32_t RBARS = BARS + (2u * NST + 2u * NACC) * 8u;  // residual boxes
+  static constexpr uint32_t MISC = RBARS + kEpiWarps * BOXES * 8u;
   static constexpr uint32_t SMEM = MISC + 16u + 1024u;  // + alignment slack
   static constexpr uint32_t TMEM_COLS = NACC * BN;
   static_assert(SMEM <= kSmemLimit, "shared memory");
-  static_assert((BN + 8u * kMaxSplits) * kTileRows * 4u <= NST * STAGE, "exchange buffer");
+  // the ring and, behind it, the boxes, which K splits do not use
+  static_assert((BN + 8u * kMaxSplits) * kTileRows * 4u <= XS, "exchange buffer");
 };
 
 struct Args {
   Fp8CodesArgs a;
-  CUtensorMap wmap, xmap, ymap;
-  bool tma_y;  // outputs by way of ymap: no residual, rows at 16-byte boundaries
+  CUtensorMap wmap, xmap, ymap, rmap;
+  bool tma_y;  // outputs by way of ymap: rows at 16-byte boundaries, no residual or RES
   uint32_t row_tiles, token_tiles, stages, splits;
   uint32_t box_tokens;  // token rows that a stage loads
 };
@@ -123,9 +127,9 @@ __device__ __forceinline__ void tile_of(const Args &A, uint32_t u, uint32_t &row
   token_tile = g * kTokenGroup + in % width;
 }
 
-template <bool PAIR>
+template <bool PAIR, bool RES>
 __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant__ Args A) {
-  using C = Cfg<PAIR>;
+  using C = Cfg<PAIR, RES>;
   constexpr uint32_t NST = C::NST, NACC = C::NACC, BN = C::BN, CH = C::COLS / 32u;
   const Fp8CodesArgs &a = A.a;
   extern __shared__ uint8_t smem_raw[];
@@ -154,6 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       mbar_init(&sh.tfull[i], 1);                  // commit after a block's MMAs
       mbar_init(&sh.tempty[i], CTAS * kEpiWarps);  // PAIR: the leading CTA's, both CTAs' warps
     }
+    for (uint32_t i = 0; i < kEpiWarps * C::BOXES; ++i) mbar_init(reinterpret_cast<uint64_t *>(smem + C::RBARS) + i, 1);
     *sh.abort = 0;
     mbar_fence_init();
   }
@@ -189,14 +194,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
   const uint32_t total = A.row_tiles * A.token_tiles;
   const uint32_t u_begin = blockIdx.x / (CTAS * splits), u_step = gridDim.x / (CTAS * splits);
   const uint32_t st0 = A.stages * split / splits, st1 = A.stages * (split + 1u) / splits;
-  const uint32_t kb0 = st0 * C::KBS, kb1 = min(st1 * C::KBS, kblocks);  // its column blocks
   const bool qkv = a.layout != PW_LAYOUT_PLAIN;
 
   if (warp < (uint32_t)kEpiWarp0) {
     if (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == (uint32_t)kProducerWarp) {
       uint32_t slot = 0, phase = 0, issued = 0, parity = 0;
-      const uint32_t bytes = C::B_BYTES + C::KBS * A.box_tokens * 128u;
+      const uint32_t bytes = C::B_BYTES + A.box_tokens * 128u;
       for (uint32_t u = u_begin; u < total; u += u_step) {
         uint32_t rt, tt;
         tile_of(A, u, rt, tt);
@@ -211,31 +215,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         for (uint32_t st = st0; st < st1; ++st) {
           if (bounded_wait(sh.abort, &sh.empty[slot], phase ^ 1u, a.flags)) {
             uint8_t *dst = sh.ring + slot * C::STAGE;
-            const int kb = (int)(st * C::KBS);
+            const int kb = (int)st;
             if (elect_one()) {
               if (PAIR) {
                 const uint32_t bar = map_rank(smem_addr(&sh.full[slot]), lead);
                 if (rank == 0u) mbar_arrive_expect_tx(&sh.full[slot], 2u * bytes);
                 tma_load_pair(dst, &A.xmap, 0, tok0, kb, bar);
-                if (!qkv) {
-                  tma_load_pair(dst + C::A_BYTES, &A.wmap, 0, (int)src0, kb, bar);
-                } else {
-                  tma_load_pair(dst + C::A_BYTES, &A.wmap, 0, (int)src0, kb, bar);
-                  tma_load_pair(dst + C::A_BYTES + 64u * 128u, &A.wmap, 0, (int)src1, kb, bar);
-                }
+                tma_load_pair(dst + C::A_BYTES, &A.wmap, 0, (int)src0, kb, bar);
+                if (qkv) tma_load_pair(dst + C::A_BYTES + 64u * 128u, &A.wmap, 0, (int)src1, kb, bar);
               } else {
                 mbar_arrive_expect_tx(&sh.full[slot], bytes);
                 tc::tma_load_3d(dst, &A.xmap, 0, tok0, kb, &sh.full[slot]);
-                if (!qkv) {
-                  tc::tma_load_3d(dst + C::A_BYTES, &A.wmap, 0, (int)src0, kb, &sh.full[slot]);
-                } else {
-#pragma unroll
-                  for (int j = 0; j < (int)C::KBS; ++j) {
-                    uint8_t *d = dst + C::A_BYTES + j * (128u * 128u);
-                    tc::tma_load_3d(d, &A.wmap, 0, (int)src0, kb + j, &sh.full[slot]);
-                    tc::tma_load_3d(d + 64u * 128u, &A.wmap, 0, (int)src1, kb + j, &sh.full[slot]);
-                  }
-                }
+                tc::tma_load_3d(dst + C::A_BYTES, &A.wmap, 0, (int)src0, kb, &sh.full[slot]);
+                if (qkv) tc::tma_load_3d(dst + C::A_BYTES + 64u * 128u, &A.wmap, 0, (int)src1, kb, &sh.full[slot]);
               }
             }
             __syncwarp();
@@ -262,28 +254,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         for (uint32_t st = st0; st < st1; ++st) {
           const bool ok_full = bounded_wait(sh.abort, &sh.full[slot], phase, a.flags);
           tc_fence_after();
+          const bool ok = bounded_wait<PAIR>(sh.abort, &sh.tempty[acc], aphase ^ 1u, a.flags) && ok_full;
+          tc_fence_after();
+          if (ok) {
+            const uint32_t d = tmem + acc * BN;
+            const uint64_t ad = ring_desc + ((slot * C::STAGE) >> 4);
+            const uint64_t bd = ad + (C::A_BYTES >> 4);
 #pragma unroll
-          for (uint32_t j = 0; j < C::KBS; ++j) {
-            if (st * C::KBS + j >= kblocks) break;
-            const bool ok = bounded_wait<PAIR>(sh.abort, &sh.tempty[acc], aphase ^ 1u, a.flags) && ok_full;
-            tc_fence_after();
-            if (ok) {
-              const uint32_t d = tmem + acc * BN;
-              // codes: a block's box_tokens rows follow one another; weights: 128 rows
-              const uint64_t ad = ring_desc + ((slot * C::STAGE + j * A.box_tokens * 128u) >> 4);
-              const uint64_t bd = ring_desc + ((slot * C::STAGE + C::A_BYTES + j * 128u * 128u) >> 4);
-#pragma unroll
-              for (uint32_t s = 0; s < 4; ++s) mma_f8<PAIR>(d, ad + 2u * s, bd + 2u * s, idesc, s ? 1u : 0u);
-            }
-            mma_commit<PAIR>(&sh.tfull[acc], 3u << lead);
-            pending |= 1u << acc;
-            pend_parity = (pend_parity & ~(1u << acc)) | (aphase << acc);
-            if (++acc == NACC) {
-              acc = 0;
-              aphase ^= 1u;
-            }
+            for (uint32_t s = 0; s < 4; ++s) mma_f8<PAIR>(d, ad + 2u * s, bd + 2u * s, idesc, s ? 1u : 0u);
           }
+          mma_commit<PAIR>(&sh.tfull[acc], 3u << lead);
           mma_commit<PAIR>(&sh.empty[slot], 3u << lead);
+          pending |= 1u << acc;
+          pend_parity = (pend_parity & ~(1u << acc)) | (aphase << acc);
+          if (++acc == NACC) {
+            acc = 0;
+            aphase ^= 1u;
+          }
           if (++slot == NST) {
             slot = 0;
             phase ^= 1u;
@@ -339,6 +326,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
     const uint32_t tempty_lead = map_rank(smem_addr(sh.tempty), cta & ~(CTAS - 1u));  // the leading CTA's
     const bool quad_r = quad_access(a.ep.residual, a.ep.residual_stride, a.ep.residual_dtype);
     const bool quad_y = quad_access(a.ep.y, a.ep.y_stride, a.ep.y_dtype);
+    // this warp's output boxes: 32 tokens x 64 bytes, `box` counts them over all tiles
+    const uint32_t box_cols = a.ep.y_dtype == PW_DTYPE_F32 ? 16u : 32u, per_tile = C::COLS / box_cols;
+    const uint32_t stg = smem_addr(smem + C::STG + (warp - kEpiWarp0) * (C::BOXES * 2048u));
+    uint64_t *rbar = reinterpret_cast<uint64_t *>(smem + C::RBARS) + (warp - kEpiWarp0) * C::BOXES;
+    uint32_t box = 0;
+    auto fetch_box = [&](uint32_t b, uint32_t col, uint32_t tok) {  // its residual
+      const uint32_t slot = b % C::BOXES;
+      mbar_arrive_expect_tx(rbar + slot, 2048u);
+      tma_load_2d(stg + slot * 2048u, &A.rmap, (int)col, (int)tok, rbar + slot);
+    };
     uint32_t acc_slot = 0, aphase = 0, ti = 0;
     float wn0 = 0.0f, wn1 = 0.0f;
     if (u_begin < total) {
@@ -353,7 +350,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       const uint32_t c_base = rt * BN + col0;  // the warp's first output column
       const bool active = rows_here != 0u && c_base < a.rows;
       tc::cp_async_wait_all();
-      if (!PAIR && lane == 0) tma_store_wait_read<0>();  // the last tile's outputs have left the other buffer
       named_bar_sync(2u + quarter, 64u);  // this tile's scales are here, the other buffer is free
       float *xsb = sh.xs + ((ti & 1u) * 4u + quarter) * (kMaxBlocks * 32u);
       const uint32_t xs_at = smem_addr(xsb + lane);
@@ -361,6 +357,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       const float wc0 = wn0, wc1 = wn1;
       if (u + u_step < total) ws_load(u + u_step, wn0, wn1);
 
+      if (RES && active && lane == 0) {
+        tma_store_wait_read<0>();  // the last tile's outputs have left the boxes
+        for (uint32_t i = 0; i < C::BOXES && i < per_tile; ++i) fetch_box(box + i, c_base + i * box_cols, tok_q);
+      }
       float acc[C::COLS];
 #pragma unroll
       for (uint32_t i = 0; i < C::COLS; ++i) acc[i] = 0.0f;
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
           s0 = __fmul_rn(__uint_as_float(p0), __uint_as_float(x1));
           s1 = CH > 2u ? __fmul_rn(__uint_as_float(p1), __uint_as_float(x1)) : s0;
         };
-        ask(kb0);
+        ask(st0);
         bounded_wait(sh.abort, &sh.tfull[acc_slot], aphase, a.flags);
         __syncwarp();
         tc_fence_after();
@@ -390,8 +390,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         answer();
         tc::tmem_wait_ld(v[0]);
 #pragma unroll 1
-        for (uint32_t kb = kb0; kb < kb1; ++kb) {
-          const bool more = kb + 1u < kb1;
+        for (uint32_t kb = st0; kb < st1; ++kb) {
+          const bool more = kb + 1u < st1;
 #pragma unroll
           for (uint32_t q = 0; q < CH; ++q) {
             const float s = q < 2u ? s0 : s1;
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         }
       } else {
         // no tokens or no rows here: keep the accumulators' handshake
-        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+        for (uint32_t kb = st0; kb < st1; ++kb) {
           bounded_wait(sh.abort, &sh.tfull[acc_slot], aphase, a.flags);
           tc_fence_after();
           tc_fence_before();
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         }
       }
 
-      if (splits > 1u) {
+      if (!RES && splits > 1u) {
         const Exchange x(sh.ring, splits, split, CTAS, rank, min(BN, a.rows - rt * BN));
         __syncwarp();
         cluster_sync_all();  // every CTA's MMAs have read their last stage
@@ -487,36 +487,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
             ok = finish_quads(a.ep, now, v, cur_bias, cur, quad_r, quad_y) && ok;
           }
         if (!ok) raise_flag(a.flags, PW_FLAG_NONFINITE_ROUND);
-      } else if (A.tma_y) {
-        // Each thread packs its token's next 32 columns into a 64-byte row of a box
-        // (two boxes of f32; 16-byte chunk i at position i ^ ((token >> 1) & 3)), which
-        // leaves by TMA while the next is made.  The loop is rolled (the sums move down
-        // 32 registers per turn): unrolled, its code left the instruction cache and a
-        // tile's epilogue took as long as its products.
+      } else if (RES || A.tma_y) {
+        // Each thread packs its token's next columns into a 64-byte row of a box (16-byte
+        // chunk i at position i ^ ((token >> 1) & 3)), which leaves by TMA while the next is
+        // made; the residual came into the same place by TMA while the products ran.  The
+        // loop is rolled (the sums move down 32 registers per turn): unrolled, its code left
+        // the instruction cache and a tile's epilogue took as long as its products.
         // lane l loads the bias of the warp's columns 4 l .. 4 l + 3
         float4 biasc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (active && 4u * lane < C::COLS) biasc = bias4(a.ep, c_base + 4u * lane);
-        if (!PAIR) named_bar_sync(2u + quarter, 64u);  // both warps are done with the scales
         if (active) {
-          const uint32_t stg = PAIR ? smem_addr(smem + C::STG + (warp - kEpiWarp0) * (C::BOXES * 2048u))
-                                    : smem_addr(xsb) + half * 2048u;
-          uint32_t box = 0;
           float most = 0.0f;
-          auto put = [&](uint32_t col, const uint4(&w)[4]) {
-            if (lane == 0) tma_store_wait_read<C::BOXES - 1u>();
-            __syncwarp();
-            const uint32_t to = stg + box * 2048u;
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + lane * 64u +
-                                                                            ((i ^ ((lane >> 1) & 3u)) << 4)),
-                           "r"(w[i].x), "r"(w[i].y), "r"(w[i].z), "r"(w[i].w)
-                           : "memory");
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) tma_store(&A.ymap, (int)col, (int)tok_q, to);
-            if (C::BOXES > 1u) box ^= 1u;
-          };
+          const uint32_t box_end = box + per_tile;
 #pragma unroll 1
           for (uint32_t h = 0; h < C::COLS / 32u; ++h) {
             float v[32];
@@ -532,23 +514,58 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
               }
             }
             activate_all(v, a.ep.act);
-#pragma unroll
-            for (uint32_t i = 0; i < 32; i += 2) most = max_abs(most, v[i], v[i + 1u]);
-            const uint32_t col = c_base + 32u * h;
-            uint4 w[4];
-            if (a.ep.y_dtype == PW_DTYPE_F32) {
-#pragma unroll
-              for (uint32_t b = 0; b < 2; ++b) {
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i)
-                  w[i] = make_uint4(__float_as_uint(v[16u * b + 4u * i]), __float_as_uint(v[16u * b + 4u * i + 1u]),
-                                    __float_as_uint(v[16u * b + 4u * i + 2u]), __float_as_uint(v[16u * b + 4u * i + 3u]));
-                put(col + 16u * b, w);
+            // a box: 16 columns of f32 from v[16 part], else all 32
+            auto put = [&](uint32_t part, bool wide) {
+              const uint32_t slot = box % C::BOXES, to = stg + slot * 2048u;
+              if (RES) {
+                // waits on its own limit: the copy lands before the CTA can exit
+                if (!mbar_wait(rbar + slot, (box / C::BOXES) & 1u)) raise_flag(a.flags, PW_FLAG_WAIT_TIMEOUT);
+              } else if (lane == 0) {
+                tma_store_wait_read<C::BOXES - 1u>();
               }
-            } else {
+              __syncwarp();
 #pragma unroll
-              for (uint32_t i = 0; i < 4; ++i) w[i] = pack8(v + 8u * i, a.ep.y_dtype);
-              put(col, w);
+              for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t at = to + lane * 64u + ((i ^ ((lane >> 1) & 3u)) << 4);
+                float *x = wide ? v + 16u * part + 4u * i : v + 8u * i;
+                uint4 q;
+                if (RES) {
+                  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                               : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                               : "r"(at));
+                  if (wide)
+                    x[0] += __uint_as_float(q.x), x[1] += __uint_as_float(q.y), x[2] += __uint_as_float(q.z),
+                        x[3] += __uint_as_float(q.w);
+                  else
+                    add8(x, q, a.ep.residual_dtype);
+                }
+                most = max_abs(max_abs(most, x[0], x[1]), x[2], x[3]);
+                if (wide) {
+                  q = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+                } else {
+                  most = max_abs(max_abs(most, x[4], x[5]), x[6], x[7]);
+                  q = pack8(x, a.ep.y_dtype);
+                }
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w)
+                             : "memory");
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) {
+                tma_store(&A.ymap, (int)(c_base + 32u * h + 16u * part), (int)tok_q, to);
+                // the box before it has left, if only just: the residual of the one that follows there
+                if (RES && box + C::BOXES - 1u < box_end && box + per_tile > box_end) {
+                  tma_store_wait_read<1>();
+                  fetch_box(box + C::BOXES - 1u, c_base + (box + C::BOXES - 1u + per_tile - box_end) * box_cols, tok_q);
+                }
+              }
+              ++box;
+            };
+            if (a.ep.y_dtype == PW_DTYPE_F32) {
+              put(0u, true);
+              put(1u, true);
+            } else {
+              put(0u, false);
             }
 #pragma unroll
             for (uint32_t i = 0; i + 32u < C::COLS; ++i) acc[i] = acc[i + 32u];
@@ -631,33 +648,42 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
 // Tiles, column blocks and the best K split of a kernel on these sizes.
 template <bool PAIR>
 Splits plan(const Fp8CodesArgs &a, int num_sms, uint32_t &row_tiles, uint32_t &token_tiles, uint32_t &stages) {
-  using C = Cfg<PAIR>;
+  using C = Cfg<PAIR, false>;
   constexpr uint32_t CTAS = PAIR ? 2u : 1u, kTokens = CTAS * kTileRows;
   row_tiles = (a.rows + C::BN - 1u) / C::BN;
   token_tiles = (a.width + kTokens - 1u) / kTokens;
-  stages = (a.K / 128u + C::KBS - 1u) / C::KBS;
-  return best_splits<k_fp8_gemm<PAIR>>(PAIR ? kCostPair : kCostOne, (uint64_t)row_tiles * token_tiles, stages * C::KBS,
-                                       kMaxSplits / CTAS, CTAS, kThreads, C::SMEM, num_sms);
+  stages = a.K / 128u;
+  return best_splits<k_fp8_gemm<PAIR, false>>(PAIR ? kCostPair : kCostOne, (uint64_t)row_tiles * token_tiles, stages,
+                                              kMaxSplits / CTAS, CTAS, kThreads, C::SMEM, num_sms);
 }
 
 // Raises the kernel's shared-memory limit, without which its occupancy is none.
-template <bool PAIR>
+template <bool PAIR, bool RES>
 cudaError_t prepare() {
-  cudaError_t e = allow_smem<k_fp8_gemm<PAIR>>(Cfg<PAIR>::SMEM);
+  cudaError_t e = allow_smem<k_fp8_gemm<PAIR, RES>>(Cfg<PAIR, RES>::SMEM);
   if (e != cudaSuccess || !PAIR) return e;
   // the register split must fit what the launch allocates, or setmaxnreg would wait for good
   static std::atomic<int> regs{0};
   if (regs.load(std::memory_order_relaxed) == 0) {
     cudaFuncAttributes at;
-    if ((e = cudaFuncGetAttributes(&at, k_fp8_gemm<PAIR>)) != cudaSuccess) return e;
+    if ((e = cudaFuncGetAttributes(&at, k_fp8_gemm<PAIR, RES>)) != cudaSuccess) return e;
     regs.store(at.numRegs, std::memory_order_relaxed);
   }
   return regs.load(std::memory_order_relaxed) < kRegsLaunch ? cudaErrorInvalidConfiguration : cudaSuccess;
 }
 
+template <bool PAIR, bool RES>
+cudaError_t launch_as(const Args &A, uint32_t clusters, cudaStream_t stream) {
+  constexpr uint32_t CTAS = PAIR ? 2u : 1u;
+  cudaError_t e = prepare<PAIR, RES>();
+  if (e != cudaSuccess) return e;
+  Launch l(CTAS * clusters, kThreads, CTAS * A.splits, Cfg<PAIR, RES>::SMEM, stream);
+  e = cudaLaunchKernelEx(&l.cfg, k_fp8_gemm<PAIR, RES>, A);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
 template <bool PAIR>
 cudaError_t launch_one(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream) {
-  using C = Cfg<PAIR>;
   constexpr uint32_t CTAS = PAIR ? 2u : 1u;
   Args A{};
   A.a = a;
@@ -665,17 +691,24 @@ cudaError_t launch_one(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream) 
   const bool qkv = a.layout != PW_LAYOUT_PLAIN;
   // up to 128 tokens a stage loads whole 32-token chunks of them
   A.box_tokens = a.width > 96u ? 128u : (a.width + 31u) / 32u * 32u;
-  if (!encode_weight_map(&A.wmap, a.w, a.rows, a.K, qkv ? 64u : 128u, qkv ? 1u : C::KBS) ||
-      !encode_weight_map(&A.xmap, a.codes, a.width, a.K, A.box_tokens, C::KBS))
+  if (!encode_weight_map(&A.wmap, a.w, a.rows, a.K, qkv ? 64u : 128u, 1u) ||
+      !encode_weight_map(&A.xmap, a.codes, a.width, a.K, A.box_tokens, 1u))
     return cudaErrorInvalidValue;
-  A.tma_y = a.ep.residual == nullptr && reinterpret_cast<uintptr_t>(a.ep.y) % 16u == 0u &&
-            encode_out_map(&A.ymap, a.ep.y, a.width, a.rows, a.ep.y_stride, a.ep.y_dtype, 32u);
   const uint64_t tiles = (uint64_t)A.row_tiles * A.token_tiles, at_once = (uint64_t)num_sms / CTAS;
   if (tiles > 0x7fffffffull / kMaxSplits) return cudaErrorInvalidValue;
   const uint32_t clusters = (uint32_t)(A.splits > 1u ? tiles * A.splits : tiles < at_once ? tiles : at_once);
-  Launch l(CTAS * clusters, kThreads, CTAS * A.splits, C::SMEM, stream);
-  cudaError_t e = cudaLaunchKernelEx(&l.cfg, k_fp8_gemm<PAIR>, A);
-  return e != cudaSuccess ? e : cudaGetLastError();
+  bool res = false;
+  if (A.splits == 1u) {
+    const auto fits = [&](CUtensorMap *map, const void *at, uint64_t stride, uint32_t dtype) {
+      return reinterpret_cast<uintptr_t>(at) % 16u == 0u && encode_out_map(map, at, a.width, a.rows, stride, dtype, 32u);
+    };
+    const bool y = fits(&A.ymap, a.ep.y, a.ep.y_stride, a.ep.y_dtype);
+    // the sums join the residual in its place: elements of one size
+    res = y && a.ep.residual && (a.ep.residual_dtype == PW_DTYPE_F32) == (a.ep.y_dtype == PW_DTYPE_F32) &&
+          fits(&A.rmap, a.ep.residual, a.ep.residual_stride, a.ep.residual_dtype);
+    A.tma_y = y && (res || !a.ep.residual);
+  }
+  return res ? launch_as<PAIR, true>(A, clusters, stream) : launch_as<PAIR, false>(A, clusters, stream);
 }
 
 }  // namespace fp8g
@@ -684,7 +717,7 @@ cudaError_t launch_fp8_gemm(const Fp8CodesArgs &a, int num_sms, cudaStream_t str
   using namespace fp8g;
   if (a.width == 0 || a.rows % 64u || a.K == 0 || a.K % 128u || a.K > 128u * kMaxBlocks) return cudaErrorInvalidValue;
   cudaError_t e;
-  if ((e = prepare<false>()) != cudaSuccess || (e = prepare<true>()) != cudaSuccess) return e;
+  if ((e = prepare<false, false>()) != cudaSuccess || (e = prepare<true, false>()) != cudaSuccess) return e;
   uint32_t r, t, s;
   if (a.width <= 128u || plan<false>(a, num_sms, r, t, s).cost <= plan<true>(a, num_sms, r, t, s).cost)
     return launch_one<false>(a, num_sms, stream);
