@@ -328,13 +328,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
     const bool quad_y = quad_access(a.ep.y, a.ep.y_stride, a.ep.y_dtype);
     // this warp's output boxes: 32 tokens x 64 bytes, `box` counts them over all tiles
     const uint32_t box_cols = a.ep.y_dtype == PW_DTYPE_F32 ? 16u : 32u, per_tile = C::COLS / box_cols;
-    const uint32_t stg = smem_addr(smem + C::STG + (warp - kEpiWarp0) * (C::BOXES * 2048u));
-    uint64_t *rbar = reinterpret_cast<uint64_t *>(smem + C::RBARS) + (warp - kEpiWarp0) * C::BOXES;
     uint32_t box = 0;
-    auto fetch_box = [&](uint32_t b, uint32_t col, uint32_t tok) {  // its residual
-      const uint32_t slot = b % C::BOXES;
-      mbar_arrive_expect_tx(rbar + slot, 2048u);
-      tma_load_2d(stg + slot * 2048u, &A.rmap, (int)col, (int)tok, rbar + slot);
+    const auto box_at = [&](uint32_t b) {
+      return smem_addr(smem + C::STG) + ((warp - kEpiWarp0) * C::BOXES + b % C::BOXES) * 2048u;
+    };
+    const auto box_bar = [&](uint32_t b) {
+      return reinterpret_cast<uint64_t *>(smem + C::RBARS) + (warp - kEpiWarp0) * C::BOXES + b % C::BOXES;
+    };
+    const auto fetch_box = [&](uint32_t b, uint32_t col, uint32_t tok) {  // its residual
+      mbar_arrive_expect_tx(box_bar(b), 2048u);
+      tma_load_2d(box_at(b), &A.rmap, (int)col, (int)tok, box_bar(b));
     };
     uint32_t acc_slot = 0, aphase = 0, ti = 0;
     float wn0 = 0.0f, wn1 = 0.0f;
@@ -498,6 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         if (active && 4u * lane < C::COLS) biasc = bias4(a.ep, c_base + 4u * lane);
         if (active) {
           float most = 0.0f;
+          if (!RES) box = 0;  // a tile's boxes are a multiple of BOXES
           const uint32_t box_end = box + per_tile;
 #pragma unroll 1
           for (uint32_t h = 0; h < C::COLS / 32u; ++h) {
@@ -516,10 +520,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
             activate_all(v, a.ep.act);
             // a box: 16 columns of f32 from v[16 part], else all 32
             auto put = [&](uint32_t part, bool wide) {
-              const uint32_t slot = box % C::BOXES, to = stg + slot * 2048u;
+              const uint32_t to = box_at(box);
               if (RES) {
                 // waits on its own limit: the copy lands before the CTA can exit
-                if (!mbar_wait(rbar + slot, (box / C::BOXES) & 1u)) raise_flag(a.flags, PW_FLAG_WAIT_TIMEOUT);
+                if (!mbar_wait(box_bar(box), (box / C::BOXES) & 1u)) raise_flag(a.flags, PW_FLAG_WAIT_TIMEOUT);
               } else if (lane == 0) {
                 tma_store_wait_read<C::BOXES - 1u>();
               }
