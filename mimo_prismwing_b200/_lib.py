@@ -7,6 +7,7 @@ its CUDA runtime and NCCL are the ones resolved in this process.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import re
 
@@ -15,9 +16,11 @@ import torch  # noqa: F401  (load order: torch's CUDA libraries first)
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 LIB_PATH = os.path.join(PKG, "lib", "libpw_cuda.so")
+BINDING_PATH = os.path.join(PKG, "lib", "_pw_torch.so")
 HEADER = os.path.join(ROOT, "include", "pw_cuda.h")
 
 _lib = None
+_binding = None
 
 
 def header_symbols(path: str = HEADER) -> list[str]:
@@ -70,6 +73,18 @@ def _bind(L: ctypes.CDLL) -> None:
     L.pw_last_profile.argtypes = [vp, vp]
     for name in header_symbols():
         getattr(L, name)  # raises AttributeError if an entry point is missing
+
+
+def binding():
+    """The compiled host side of the calls on torch tensors (binding/pw_torch.cpp)."""
+    global _binding
+    if _binding is None:
+        if not os.path.exists(BINDING_PATH):
+            raise RuntimeError(f"{BINDING_PATH} is missing: build it with `python -m mimo_prismwing_b200.build`")
+        spec = importlib.util.spec_from_file_location("_pw_torch", BINDING_PATH)
+        _binding = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_binding)
+    return _binding
 
 
 def load() -> ctypes.CDLL:
