@@ -2,10 +2,11 @@
 //
 // For a single token these calls take 2 to 11 us on the device, and Python code that
 // looks at every tensor, allocates the outputs and goes through ctypes took 9.5 to 14.5
-// us per call (4.5 to 7.5 here, 3 of them the launch); here it is an asynchronous call's checks, descriptors and allocations in
-// one step.  A call that is not the ordinary one (host rows, a shape or type to be
-// refused, a tensor subclass) is not taken: the methods return None and the
-// caller's own path, which words the refusals, runs.  A status is returned as an int.
+// us per call (4.5 to 7.5 here, 3 of them the launch).  Here an asynchronous call's
+// checks, descriptors and allocations are one step.  A call that is not the ordinary
+// one (host rows, a shape or type to be refused, a tensor subclass) is not taken: the
+// methods return None and the caller's own path, which words the refusals, runs.  A
+// status is returned as an int.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
