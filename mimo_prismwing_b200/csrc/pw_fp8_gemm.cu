@@ -56,7 +56,7 @@ constexpr uint32_t kMaxBlocks = 32;   // K <= 4096
 // 2048 10.1 / 10.8, 64 x 4096 x 4096 15.8 / 11.0.
 constexpr TileCost kCostOne{800u, 6000u, 13500u}, kCostPair{1150u, 9000u, 28000u};
 constexpr uint32_t kTokenGroup = 8;   // token tiles that neighbouring pairs share weights over
-// Register split of PAIR: 256 x 240 + 128 x 24, all of the 384 x 168 at launch.
+// Register split: 256 x 240 + 128 x 24, all of the 384 x 168 at launch.
 constexpr int kRegsLaunch = 168, kRegsEpi = 240, kRegsOther = 24;
 static_assert(kEpiWarps * 32 * kRegsEpi + kEpiWarp0 * 32 * kRegsOther <= kThreads * kRegsLaunch, "register split");
 
@@ -71,11 +71,13 @@ struct Cfg {
   static constexpr uint32_t STAGE = A_BYTES + B_BYTES;
   static constexpr uint32_t NST = RES ? 4u : 5u;
   static constexpr uint32_t NACC = PAIR ? 2u : 4u;
+  static constexpr uint32_t G = PAIR ? 2u : 4u;  // blocks whose scales are fetched together, as registers allow
   static constexpr uint32_t COLS = BN / 2u;  // a thread's columns: two warps per lane quarter
   static constexpr uint32_t BOXES = RES ? 4u : 2u;  // 2 KB output boxes per epilogue warp
   static constexpr uint32_t STG = NST * STAGE;
-  static constexpr uint32_t XS = STG + kEpiWarps * BOXES * 2048u;  // token scales [2 tiles][4 quarters][32 blocks][32 tokens] f32
-  static constexpr uint32_t BARS = XS + 2u * 4u * kMaxBlocks * 32u * 4u;
+  static constexpr uint32_t XS = STG + kEpiWarps * BOXES * 2048u;  // token scales [2 tiles][4 quarters][32 tokens][32 blocks] f32
+  static constexpr uint32_t WS = XS + 2u * 4u * 32u * kMaxBlocks * 4u;  // weight scales [2 tiles][BN / 64 runs of rows][32 blocks]
+  static constexpr uint32_t BARS = WS + 2u * (BN / 64u) * kMaxBlocks * 4u;
   static constexpr uint32_t RBARS = BARS + (2u * NST + 2u * NACC) * 8u;  // residual boxes
   static constexpr uint32_t MISC = RBARS + kEpiWarps * BOXES * 8u;
   static constexpr uint32_t SMEM = MISC + 16u + 1024u;  // + alignment slack
@@ -118,6 +120,13 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(accum)
         : "memory");
+}
+
+__device__ __forceinline__ void lds(float (&v)[4], uint32_t at) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(at));
+}
+__device__ __forceinline__ void lds(float (&v)[2], uint32_t at) {
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(at));
 }
 
 __device__ __forceinline__ void tile_of(const Args &A, uint32_t u, uint32_t &row_tile, uint32_t &token_tile) {
@@ -197,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
   const bool qkv = a.layout != PW_LAYOUT_PLAIN;
 
   if (warp < (uint32_t)kEpiWarp0) {
-    if (PAIR) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == (uint32_t)kProducerWarp) {
       uint32_t slot = 0, phase = 0, issued = 0, parity = 0;
       const uint32_t bytes = C::B_BYTES + A.box_tokens * 128u;
@@ -290,38 +299,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       cluster_sync_all();
     }
   } else {
-    if (PAIR) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     // two warps per TMEM lane quarter: 32 tokens, half of the tile's columns each
     const uint32_t quarter = warp % 4u, half = (warp - kEpiWarp0) / 4u, col0 = half * C::COLS;
     const uint32_t row = quarter * 32u + lane;  // this thread's token of the CTA
     const uint32_t cols = tmem + ((quarter * 32u) << 16) + col0;
-    // Token scales: the quarter's two warps copy its 32 tokens' ([block][token]:
-    // read by lane without conflicts) for the next tile while this one runs.
-    auto xs_fetch = [&](uint32_t u, uint32_t buf) {
-      uint32_t rt, tt;
+    // The next tile's scales are copied while this one runs: token scales by the
+    // quarter's two warps, a row of 32 blocks per token (G blocks i at position i ^
+    // token: a lane's G blocks are one load without conflicts); weight scales, per 64
+    // rows, by all warps.
+    const auto fetch_scales = [&](uint32_t u, uint32_t buf) {
+      uint32_t rt, tt, unused, row;
       tile_of(A, u, rt, tt);
       const uint32_t tok0 = (tt * CTAS + rank) * kTileRows + quarter * 32u;
       float *dst = sh.xs + (buf * 4u + quarter) * (kMaxBlocks * 32u);
-      for (uint32_t e = half * 32u + lane; e < 32u * kblocks; e += 64u) {
-        const uint32_t kb = e / 32u, t = e % 32u;
-        if (tok0 + t < a.width) tc::cp_async4(dst + kb * 32u + t, a.scales + (uint64_t)(tok0 + t) * kblocks + kb);
+      if (lane < kblocks)
+        for (uint32_t t = half; t < 32u && tok0 + t < a.width; t += 2u)
+          tc::cp_async4(dst + t * 32u + ((lane / C::G) ^ (t % (32u / C::G))) * C::G + lane % C::G,
+                        a.scales + (uint64_t)(tok0 + t) * kblocks + lane);
+      const uint32_t run = warp - kEpiWarp0, r = rt * BN + run * 64u;
+      if (run < BN / 64u && r < a.rows && lane < kblocks) {
+        map_row(a.layout, r, unused, row);
+        tc::cp_async4(reinterpret_cast<float *>(smem + C::WS) + (buf * (BN / 64u) + run) * 32u + lane,
+                      a.ws + (uint64_t)row * kblocks + lane);
       }
       tc::cp_async_commit();
-    };
-    // Weight scales: lane l holds block l of the scale rows of the warp's columns
-    // (64 or 128 rows of one 128-row block, or of two 64-row QKV runs).
-    auto ws_load = [&](uint32_t u, float &w0, float &w1) {
-      uint32_t rt, tt, unused, s0, s1;
-      tile_of(A, u, rt, tt);
-      const uint32_t r = rt * BN + col0;
-      w0 = w1 = 0.0f;
-      if (r >= a.rows || lane >= kblocks) return;
-      map_row(a.layout, r, unused, s0);
-      w0 = w1 = __ldg(a.ws + (uint64_t)s0 * kblocks + lane);
-      if (C::COLS > 64u && qkv) {
-        map_row(a.layout, r + 64u, unused, s1);
-        w1 = __ldg(a.ws + (uint64_t)s1 * kblocks + lane);
-      }
     };
     const uint32_t tempty_lead = map_rank(smem_addr(sh.tempty), cta & ~(CTAS - 1u));  // the leading CTA's
     const bool quad_r = quad_access(a.ep.residual, a.ep.residual_stride, a.ep.residual_dtype);
@@ -340,11 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       tma_load_2d(box_at(b), &A.rmap, (int)col, (int)tok, box_bar(b));
     };
     uint32_t acc_slot = 0, aphase = 0, ti = 0;
-    float wn0 = 0.0f, wn1 = 0.0f;
-    if (u_begin < total) {
-      ws_load(u_begin, wn0, wn1);
-      xs_fetch(u_begin, 0u);
-    }
+    if (u_begin < total) fetch_scales(u_begin, 0u);
     for (uint32_t u = u_begin; u < total; u += u_step, ++ti) {
       uint32_t rt, tt;
       tile_of(A, u, rt, tt);
@@ -353,12 +351,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       const uint32_t c_base = rt * BN + col0;  // the warp's first output column
       const bool active = rows_here != 0u && c_base < a.rows;
       tc::cp_async_wait_all();
-      named_bar_sync(2u + quarter, 64u);  // this tile's scales are here, the other buffer is free
+      named_bar_sync(2u, kEpiWarps * 32u);  // this tile's scales are here, the other buffer is free
       float *xsb = sh.xs + ((ti & 1u) * 4u + quarter) * (kMaxBlocks * 32u);
-      const uint32_t xs_at = smem_addr(xsb + lane);
-      if (u + u_step < total) xs_fetch(u + u_step, (ti & 1u) ^ 1u);
-      const float wc0 = wn0, wc1 = wn1;
-      if (u + u_step < total) ws_load(u + u_step, wn0, wn1);
+      if (u + u_step < total) fetch_scales(u + u_step, (ti & 1u) ^ 1u);
 
       if (RES && active && lane == 0) {
         tma_store_wait_read<0>();  // the last tile's outputs have left the boxes
@@ -371,41 +366,52 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         // A chunk of 32 columns loads while the previous one is promoted; the
         // accumulator goes back to the MMA once its last chunk is in registers.  A warp
         // issues in order, so what takes long to come back is asked for early: the next
-        // block's scales at the block's start (multiplied at its end), the next
-        // accumulator's barrier half a chunk before it is needed.
+        // accumulator's barrier half a chunk before it is needed, scales G blocks at
+        // a time before the last chunk of the G (a load and two shuffles per block cost a
+        // tenth of the loop).
         float v[2][32];
-        uint32_t x1, p0, p1;  // the next block's scales: the token's, the weight's
-        auto ask = [&](uint32_t kb) {
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x1) : "r"(xs_at + kb * 128u));
-          p0 = __shfl_sync(0xffffffffu, __float_as_uint(wc0), kb);
-          if (CH > 2u) p1 = __shfl_sync(0xffffffffu, __float_as_uint(wc1), kb);
+        float xg[C::G], wg[C::COLS / 64u][C::G], sg[C::COLS / 64u][C::G];
+        const uint32_t xs_at = smem_addr(xsb) + lane * 128u;
+        const uint32_t ws_at = smem_addr(smem + C::WS) + (((ti & 1u) * (BN / 64u) + half * (C::COLS / 64u)) * 128u);
+        const auto ask = [&](uint32_t kb) {  // for the G blocks around kb
+          lds(xg, xs_at + ((kb / C::G) ^ (lane % (32u / C::G))) * (4u * C::G));
+#pragma unroll
+          for (uint32_t h = 0; h < C::COLS / 64u; ++h) lds(wg[h], ws_at + h * 128u + (kb / C::G) * (4u * C::G));
         };
-        float s0, s1;
-        auto answer = [&]() {
-          s0 = __fmul_rn(__uint_as_float(p0), __uint_as_float(x1));
-          s1 = CH > 2u ? __fmul_rn(__uint_as_float(p1), __uint_as_float(x1)) : s0;
+        const auto answer = [&]() {
+#pragma unroll
+          for (uint32_t h = 0; h < C::COLS / 64u; ++h)
+#pragma unroll
+            for (uint32_t i = 0; i < C::G; ++i) sg[h][i] = __fmul_rn(wg[h][i], xg[i]);
+        };
+        const auto next_scale = [&]() {
+#pragma unroll
+          for (uint32_t h = 0; h < C::COLS / 64u; ++h)
+#pragma unroll
+            for (uint32_t i = 0; i + 1u < C::G; ++i) sg[h][i] = sg[h][i + 1u];
         };
         ask(st0);
+        answer();
+        for (uint32_t i = 0; i < st0 % C::G; ++i) next_scale();
         bounded_wait(sh.abort, &sh.tfull[acc_slot], aphase, a.flags);
         __syncwarp();
         tc_fence_after();
         tc::tmem_ld32(cols + acc_slot * BN, v[0]);
-        answer();
         tc::tmem_wait_ld(v[0]);
 #pragma unroll 1
         for (uint32_t kb = st0; kb < st1; ++kb) {
           const bool more = kb + 1u < st1;
 #pragma unroll
           for (uint32_t q = 0; q < CH; ++q) {
-            const float s = q < 2u ? s0 : s1;
+            const float s = sg[q / 2u][0];
             float(&now)[32] = v[q & 1u];
             float(&next)[32] = v[(q & 1u) ^ 1u];
             const bool last = q + 1u == CH;
             bool ready = true;
             if (!last) {
               tc::tmem_ld32(cols + acc_slot * BN + 32u * (q + 1u), next);
-              if (q == 0u && more) ask(kb + 1u);
             } else {
+              if (kb % C::G == C::G - 1u && more) ask(kb + 1u);
               tc_fence_before();
               __syncwarp();
               if (lane == 0) arrive_relaxed_remote(tempty_lead + acc_slot * 8u);
@@ -427,7 +433,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
             for (int i = 16; i < 32; ++i) acc[32u * q + i] = __fmaf_rn(now[i], s, acc[32u * q + i]);
             if (!last || more) tc::tmem_wait_ld(next);
           }
-          answer();
+          if (kb % C::G == C::G - 1u) answer();
+          else next_scale();
         }
       } else {
         // no tokens or no rows here: keep the accumulators' handshake
@@ -589,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         // lane l loads the bias of the warp's columns 4 l .. 4 l + 3
         float4 biasc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (active && 4u * lane < C::COLS) biasc = bias4(a.ep, c_base + 4u * lane);
-        named_bar_sync(2u + quarter, 64u);
+        named_bar_sync(3u + quarter, 64u);
         if (active) {
           uint8_t *stg = reinterpret_cast<uint8_t *>(xsb) + half * 2048u;
           const uint32_t c4 = lane % 4u, r0 = lane / 4u;
@@ -665,7 +672,7 @@ Splits plan(const Fp8CodesArgs &a, int num_sms, uint32_t &row_tiles, uint32_t &t
 template <bool PAIR, bool RES>
 cudaError_t prepare() {
   cudaError_t e = allow_smem<k_fp8_gemm<PAIR, RES>>(Cfg<PAIR, RES>::SMEM);
-  if (e != cudaSuccess || !PAIR) return e;
+  if (e != cudaSuccess) return e;
   // the register split must fit what the launch allocates, or setmaxnreg would wait for good
   static std::atomic<int> regs{0};
   if (regs.load(std::memory_order_relaxed) == 0) {
