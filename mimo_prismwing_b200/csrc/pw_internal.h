@@ -294,7 +294,7 @@ struct Fp8CodesArgs {
   EpilogueArgs ep;
   uint32_t *flags;
 };
-cudaError_t launch_fp8_narrow(const Fp8CodesArgs &a, cudaStream_t stream);  // up to 16 tokens
+cudaError_t launch_fp8_narrow(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream);  // up to 16 tokens
 cudaError_t launch_fp8_gemm(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream);
 
 // Expert-parallel window of one rank (byte offsets from its base): flags

@@ -368,7 +368,7 @@ def test_fp8_codes_match_fp8_linear(rt, width, layout):
 
 
 @pytest.mark.parametrize("width", [1, 7, 13, 33, 64, 128, 140, 256, 300, 600])
-@pytest.mark.parametrize("rows,cols", [(128, 128), (384, 640), (256, 4096), (9600, 256), (4096, 2048)])
+@pytest.mark.parametrize("rows,cols", [(128, 128), (384, 640), (256, 4096), (9600, 256), (4096, 2048), (4864, 384)])
 def test_fp8_sums_are_exact_on_small_integers(rt, width, rows, cols):
     # codes of small integers, scales powers of two: every sum is exact in f32, every index error shows
     from mimo_prismwing_b200.runtime import WideProjectionBinding
@@ -383,6 +383,29 @@ def test_fp8_sums_are_exact_on_small_integers(rt, width, rows, cols):
         (w.double() * ws.double().repeat_interleave(128, 0).repeat_interleave(128, 1)).t()
     assert torch.equal(out.double(), ref)
     assert (buf[:, rows:] == 9.0).all()
+
+
+@pytest.mark.parametrize("width", [16, 31, 128, 300, 1030])
+@pytest.mark.parametrize("rows,cols", [(128, 128), (4864, 384), (19200, 256)])
+@pytest.mark.parametrize("out,res", [("f32", "f32"), ("bf16", "bf16"), ("f16", "bf16"), ("bf16", "f32"), ("f32", "f16")])
+def test_fp8_residual_and_output_boxes(rt, width, rows, cols, out, res):
+    # small integers again, so that one rounding is all there is: many tiles per CTA,
+    # residuals of the output's element size and of the other, packed, strided and in place
+    from mimo_prismwing_b200.runtime import WideProjectionBinding
+    x = torch.randint(-3, 4, (width, cols), generator=gen(246), device="cuda").float()
+    w = torch.randint(-3, 4, (rows, cols), generator=gen(247), device="cuda").float()
+    r = torch.randint(-99, 100, (width, rows), generator=gen(248), device="cuda").to(TYPES[res])
+    bias = torch.randint(-9, 10, (rows,), generator=gen(249), device="cuda").float()
+    b = WideProjectionBinding(w.to(torch.float8_e4m3fn).view(torch.uint8), torch.ones(rows // 128, cols // 128, device="cuda"))
+    codes, scales = x.to(torch.float8_e4m3fn).view(torch.uint8), torch.ones(width, cols // 128, device="cuda")
+    ref = (x.double() @ w.double().t() + bias.double() + r.double()).to(TYPES[out])
+    kw = dict(bias=bias, out_dtype=TYPES[out])
+    assert torch.equal(rt.fp8_linear_codes(codes, scales, b, residual=r, **kw).output, ref)
+    assert torch.equal(rt.fp8_linear_codes(codes, scales, b, residual=wide(r, 16)[0], **kw).output, ref)
+    assert torch.equal(rt.fp8_linear_codes(codes, scales, b, residual=wide(r, 3)[0], **kw).output, ref)
+    if out == res:
+        rt.fp8_linear_codes(codes, scales, b, residual=r, out=r, **kw)
+        assert torch.equal(r, ref)
 
 
 @pytest.mark.parametrize("act", list(ACTS))
