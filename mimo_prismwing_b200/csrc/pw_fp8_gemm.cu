@@ -49,12 +49,12 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint32_t kSmemLimit = 227u * 1024u;
 constexpr uint32_t kMaxBlocks = 32;   // K <= 4096
-// Measured cycles (B200 at 1.9 GHz): the one-CTA tile 800 per block and 6000 per wave, a
-// pair's, of four times the products, 1150 and 9000; joining K splits costs 13500 and
-// 28000 in place of the latter.  In us, one CTA / pair: 512 x 4096 x 4096 18.0 / 24.4, 768 x
-// 4096 x 4096 33.1 / 26.3, 256 x 13568 x 4096 33.8 / 27.2; unsplit / split one-CTA tiles: 203 x 4096 x
-// 2048 10.1 / 10.8, 64 x 4096 x 4096 15.8 / 11.0.
-constexpr TileCost kCostOne{800u, 6000u, 13500u}, kCostPair{1150u, 9000u, 28000u};
+// Measured cycles (B200 at 1.9 GHz): the one-CTA tile 640 per block and 5500 per wave, a
+// pair's, of four times the products, 950 and 11000; joining K splits costs 13500 and
+// 28000 in place of the latter.  In us, one CTA / pair: 512 x 4096 x 4096 15.0 / 22.9, 768 x
+// 4096 x 4096 27.9 / 23.9, 384 x 13568 x 4096 41.0 / 43.8, 1024 x 13568 x 4096 83.6 / 65.4;
+// unsplit / split one-CTA tiles: 203 x 4096 x 2048 9.6 / 10.8, 64 x 4096 x 4096 14.4 / 9.9.
+constexpr TileCost kCostOne{640u, 5500u, 13500u}, kCostPair{950u, 11000u, 28000u};
 constexpr uint32_t kTokenGroup = 8;   // token tiles that neighbouring pairs share weights over
 // Register split: 256 x 240 + 128 x 24, all of the 384 x 168 at launch.
 constexpr int kRegsLaunch = 168, kRegsEpi = 240, kRegsOther = 24;
@@ -308,15 +308,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
     // quarter's two warps, a row of 32 blocks per token (G blocks i at position i ^
     // token: a lane's G blocks are one load without conflicts); weight scales, per 64
     // rows, by all warps.
+    const uint32_t shift = 32u - __clz(kblocks - 1u);  // 2^shift >= kblocks (__clz(0) is 32)
     const auto fetch_scales = [&](uint32_t u, uint32_t buf) {
       uint32_t rt, tt, unused, row;
       tile_of(A, u, rt, tt);
       const uint32_t tok0 = (tt * CTAS + rank) * kTileRows + quarter * 32u;
       float *dst = sh.xs + (buf * 4u + quarter) * (kMaxBlocks * 32u);
-      if (lane < kblocks)
-        for (uint32_t t = half; t < 32u && tok0 + t < a.width; t += 2u)
-          tc::cp_async4(dst + t * 32u + ((lane / C::G) ^ (t % (32u / C::G))) * C::G + lane % C::G,
-                        a.scales + (uint64_t)(tok0 + t) * kblocks + lane);
+      // 2^shift lanes per token
+      const uint32_t kb = lane & ((1u << shift) - 1u), step = 64u >> shift;
+      if (kb < kblocks)
+        for (uint32_t t = (half * 32u + lane) >> shift; t < 32u && tok0 + t < a.width; t += step)
+          tc::cp_async4(dst + t * 32u + ((kb / C::G) ^ (t % (32u / C::G))) * C::G + kb % C::G,
+                        a.scales + (uint64_t)(tok0 + t) * kblocks + kb);
       const uint32_t run = warp - kEpiWarp0, r = rt * BN + run * 64u;
       if (run < BN / 64u && r < a.rows && lane < kblocks) {
         map_row(a.layout, r, unused, row);
