@@ -101,6 +101,9 @@ __device__ __forceinline__ void tma_store_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 
+// The end of their writing.
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // One look at a barrier's phase; SLEEP: waits in hardware for up to 100 us, woken
 // by the phase's completion.  PAIR: the pair's other CTA arrives on the barrier too.
 template <bool PAIR, bool SLEEP>

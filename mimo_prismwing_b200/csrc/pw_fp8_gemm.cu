@@ -16,10 +16,11 @@
 //    per 64 cycles of products, all that shared memory gives, before TMA has
 //    written any; a pair's needs half of that.  Eight epilogue warps hold 128
 //    sums per thread: setmaxnreg moves the registers of the other four to them.
-//    What bounds it is the hand-over of the two accumulators between MMA and
-//    epilogue (2048 x 16384 x 4096 takes 200 us; 165 with an eighth of the FMAs,
-//    191 with a quarter of the MMAs, 162 with an eighth of the output passes).
-//    Sixteen warps with 64 sums each, with the registers that leaves, took 214 us.
+//    What bounds it is the promotion: a block's takes 950 cycles against 512 of
+//    products (when 2048 x 16384 x 4096 took 164 us: 126 with an eighth of the FMAs, 152
+//    with a quarter of the MMAs, 99 with both, 165 without the weights' loads).  Sixteen
+//    warps with 64 sums each, with the registers that leaves, were slower, and so were
+//    128-column accumulators, handed back by halves.
 //  * one CTA, for the widths between: 128 x 128 tiles, bound by the weight stream.  When
 //    the tiles are fewer than the SMs a cluster's CTAs split K and exchange their
 //    sums (pw_cluster.cuh).
@@ -60,9 +61,9 @@ constexpr uint32_t kTokenGroup = 8;   // token tiles that neighbouring pairs sha
 constexpr int kRegsLaunch = 168, kRegsEpi = 240, kRegsOther = 24;
 static_assert(kEpiWarps * 32 * kRegsEpi + kEpiWarp0 * 32 * kRegsOther <= kThreads * kRegsLaunch, "register split");
 
-// RES: the residual comes into the output boxes by TMA.  It takes more boxes to hide,
-// and the ring gives way (2048 x 16384 x 4096, us with / without a residual: four stages
-// and four boxes 186 / 181, five and two 190+ / 171).
+// RES: the residual comes into the output boxes by TMA (2048 x 16384 x 4096 bf16: 219 us
+// with it read and added on the way out, 184 so).  That takes four boxes per warp to
+// hide, and the ring gives way to them; without a residual four stages cost 6%.
 template <bool PAIR, bool RES>
 struct Cfg {
   static constexpr uint32_t BN = PAIR ? 256u : 128u;    // weight rows of a tile
@@ -643,7 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
     }
   }
 
-  if (warp >= (uint32_t)kEpiWarp0 && lane == 0) tma_store_wait_read<0>();
+  // the outputs are written before the grid can be complete for the kernel behind it
+  if (warp >= (uint32_t)kEpiWarp0 && lane == 0) tma_store_wait();
   tc_fence_before();
   __syncthreads();
   if (PAIR) {
