@@ -21,9 +21,10 @@
 //    with a quarter of the MMAs, 99 with both, 165 without the weights' loads).  Sixteen
 //    warps with 64 sums each, with the registers that leaves, were slower, and so were
 //    128-column accumulators, handed back by halves.
-//  * one CTA, for the widths between: 128 x 128 tiles, bound by the weight stream.  When
-//    the tiles are fewer than the SMs a cluster's CTAs split K and exchange their
-//    sums (pw_cluster.cuh).
+//  * one CTA, for the widths between: 128 x 128 tiles, 640 cycles per column block, of
+//    which shared memory takes 512 (32 KB written by TMA, 32 KB read by the MMAs); with
+//    few tokens the weight stream bounds it.  When the tiles are fewer than the SMs a
+//    cluster's CTAs split K and exchange their sums (pw_cluster.cuh).
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_runtime.h>
