@@ -227,7 +227,10 @@ int pw_runtime_create(int device, uint32_t flags, pw_runtime **out);
 void pw_runtime_destroy(pw_runtime *rt);
 /* Text of the last error on this runtime ("" if none); valid until the next call. */
 const char *pw_last_error(const pw_runtime *rt);
-/* Run subsequent calls on a caller stream (a cudaStream_t passed as void*); NULL restores the runtime's own. */
+/* Run subsequent calls on a caller stream (a cudaStream_t passed as void*); NULL restores the runtime's own.
+ * pw_add_rms_norm, pw_linear and pw_fp8_linear_codes on device rows share no memory with calls that
+ * still run on the stream before.  The other calls, and all calls on host rows, use the scratch
+ * arena: let asynchronous ones end, or make the new stream wait for them, before they follow there. */
 int pw_set_stream(pw_runtime *rt, void *cuda_stream);
 int pw_synchronize(pw_runtime *rt);
 /* Device error-flag word accumulated since the last call that reset it (0 = clean). */
@@ -338,7 +341,9 @@ int pw_add_rms_norm(pw_runtime *rt, const pw_norm *norm, const pw_rows *x, const
  * A token's result does not depend on the other tokens' values, and is the same
  * in every call of the same sizes; other sizes may add the products in another
  * order.  A captured call that converts or copies x allocates the copy in the
- * graph; no other captured call uses memory besides its arguments. */
+ * graph; no other captured call uses memory besides its arguments.  Eager calls
+ * that convert or copy x share the runtime's memory for it: on different streams
+ * they wait for one another. */
 int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t width, const pw_epilogue *ep,
               const pw_rows *y, uint32_t mem, pw_stats *stats);
 

@@ -154,6 +154,10 @@ struct pw_runtime {
   uint32_t *d_router_work = nullptr;      // router unit counters (two words, left zero)
   void *scratch = nullptr;
   size_t scratch_cap = 0;
+  // x of eager pw_linear calls as their kernels read it, and the end of the last of them
+  void *convert = nullptr;
+  size_t convert_cap = 0;
+  cudaEvent_t convert_done = nullptr;
   cudaEvent_t ev0 = nullptr, ev1 = nullptr;
   // profiling: an event before and after each timed launch group
   static constexpr int kProfEvents = 32;
@@ -267,6 +271,27 @@ int ensure_scratch(pw_runtime *rt, size_t bytes) {
   rt->scratch_cap = 0;
   CK(cudaMalloc(&rt->scratch, cap));
   rt->scratch_cap = cap;
+  return PW_OK;
+}
+
+// Memory for a pw_linear call's converted x, apart from the scratch, which asynchronous
+// calls on a stream that the runtime ran on before may still use.  Calls that share it
+// may be on different streams: each waits for the one before it, which records
+// convert_done behind its kernels.
+int ensure_convert(pw_runtime *rt, size_t bytes) {
+  if (!rt->convert_done) CK(cudaEventCreateWithFlags(&rt->convert_done, cudaEventDisableTiming));
+  if (bytes <= rt->convert_cap) {
+    CK(cudaStreamWaitEvent(rt->stream, rt->convert_done, 0));
+    return PW_OK;
+  }
+  size_t cap = rt->convert_cap ? rt->convert_cap : (size_t)1 << 16;
+  while (cap < bytes) cap *= 2;
+  CK(cudaEventSynchronize(rt->convert_done));
+  if (rt->convert) CK(cudaFree(rt->convert));
+  rt->convert = nullptr;
+  rt->convert_cap = 0;
+  CK(cudaMalloc(&rt->convert, cap));
+  rt->convert_cap = cap;
   return PW_OK;
 }
 
@@ -637,6 +662,11 @@ void pw_runtime_destroy(pw_runtime *rt) {
     delete rt->ep;
   }
   if (rt->scratch) cudaFree(rt->scratch);
+  if (rt->convert_done) {
+    cudaEventSynchronize(rt->convert_done);
+    cudaEventDestroy(rt->convert_done);
+  }
+  if (rt->convert) cudaFree(rt->convert);
   if (rt->split_ws) cudaFree(rt->split_ws);
   if (rt->split_cnt) cudaFree(rt->split_cnt);
   if (rt->silu_lut) cudaFree(rt->silu_lut);
@@ -1165,6 +1195,7 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
                                                                  xr.stride % 8u || xr.stride >= ((uint64_t)1 << 36)));
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   if (convert && !call.host()) CK(cudaStreamIsCapturing(rt->stream, &capture));
+  const bool captured = capture != cudaStreamCaptureStatusNone;
   GraphMemory graph;
   Arena ar;
   for (int pass = 0; pass < 2; ++pass) {
@@ -1182,12 +1213,14 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
     if (convert) {
       cx.dtype = w->dtype;
       Arena none;
-      cx = device_rows(capture == cudaStreamCaptureStatusNone ? ar : none, cx, width, K);
+      cx = device_rows(call.host() ? ar : none, cx, width, K);
     }
     if (pass == 0) continue;
-    if (convert && capture != cudaStreamCaptureStatusNone) {
-      CK(graph.take((size_t)width * cx.stride * 2u, rt->stream));
-      cx.data = graph.at;
+    if (convert && !call.host()) {
+      const size_t bytes = (size_t)width * cx.stride * 2u;
+      if (captured) CK(graph.take(bytes, rt->stream));
+      else if ((s = ensure_convert(rt, bytes)) != PW_OK) return s;
+      cx.data = captured ? graph.at : rt->convert;
     }
     if (call.host()) {
       CK(copy_rows(dx, xr, width, K, cudaMemcpyHostToDevice, rt->stream));
@@ -1214,7 +1247,8 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
       PdlScope pdl(!rt->profiling);
       CK(launch_linear(a, rt->num_sms, rt->stream));
     }
-    CK(graph.give());
+    if (captured) CK(graph.give());
+    else if (convert && !call.host()) CK(cudaEventRecord(rt->convert_done, rt->stream));
     if (call.host()) CK(copy_rows(yr, dy, width, N, cudaMemcpyDeviceToHost, rt->stream));
   }
   return call.finish((uint64_t)N * K * 2u);
