@@ -171,28 +171,38 @@ def prepare(case, seed):
 
 
 # ------------------------------------------------------------------ the library's calls
-_runtime = None
+_runtimes = {}  # by device: [the runtime, the stream that it runs on]
+
+
+def _runtime():
+    """The current device's runtime, on the current stream."""
+    device = torch.cuda.current_device()
+    stream = torch._C._cuda_getCurrentRawStream(device)  # torch.cuda.current_stream() takes as long as a short call
+    kept = _runtimes.get(device)
+    if kept is None:
+        from mimo_prismwing_b200.runtime import WideMoeRuntime
+        kept = _runtimes[device] = [WideMoeRuntime.compile_with_fused_gate_up(device), None]
+    if kept[1] != stream:
+        kept[0].set_stream(torch.cuda.current_stream())
+        kept[1] = stream
+    return kept[0]
 
 
 def _own(s):
-    global _runtime
-    from mimo_prismwing_b200.runtime import LAYOUT_FULL_QKV, LAYOUT_PLAIN, WideMoeRuntime, WideProjectionBinding
-    if _runtime is None:
-        _runtime = WideMoeRuntime.compile_with_fused_gate_up(torch.cuda.current_device())
-        _runtime.set_stream(torch.cuda.current_stream())
+    from mimo_prismwing_b200.runtime import LAYOUT_FULL_QKV, LAYOUT_PLAIN, WideProjectionBinding
+    rt = _runtime()
     c = s["case"]
     if c["op"] == "norm":
-        r = _runtime.add_rms_norm(s["x"], s["weight"], EPS, residual=s["residual"], want_y=c["y"],
-                                  want_codes=c["codes"], asynchronous=True)
+        r = rt.add_rms_norm(s["x"], s["weight"], EPS, residual=s["residual"], want_y=c["y"],
+                            want_codes=c["codes"], asynchronous=True)
         return _norm_outputs(c, r.sum, r.y, r.codes, r.scales)
     out = TYPES[c["out"]]
     if c["op"] == "linear":
-        return _runtime.linear(s["x"], s["weight"], bias=s["bias"], activation=c["act"], residual=s["residual"],
-                               out_dtype=out, asynchronous=True).output
-    return _runtime.fp8_linear_codes(s["codes"], s["scales"], WideProjectionBinding(s["weight"], s["weight_scale"]),
-                                     layout=LAYOUT_FULL_QKV if c["qkv"] else LAYOUT_PLAIN, bias=s["bias"],
-                                     activation=c["act"], residual=s["residual"], out_dtype=out,
-                                     asynchronous=True).output
+        return rt.linear(s["x"], s["weight"], bias=s["bias"], activation=c["act"], residual=s["residual"],
+                         out_dtype=out, asynchronous=True).output
+    return rt.fp8_linear_codes(s["codes"], s["scales"], WideProjectionBinding(s["weight"], s["weight_scale"]),
+                               layout=LAYOUT_FULL_QKV if c["qkv"] else LAYOUT_PLAIN, bias=s["bias"],
+                               activation=c["act"], residual=s["residual"], out_dtype=out, asynchronous=True).output
 
 
 def _norm_outputs(c, total, y, codes, scales):
