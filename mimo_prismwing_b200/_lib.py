@@ -10,13 +10,15 @@ import ctypes
 import importlib.util
 import os
 import re
+import sysconfig
 
 import torch  # noqa: F401  (load order: torch's CUDA libraries first)
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 LIB_PATH = os.path.join(PKG, "lib", "libpw_cuda.so")
-BINDING_PATH = os.path.join(PKG, "lib", "_pw_torch.so")
+# the extension uses torch's C++ classes and CPython's: one file per version of both
+BINDING_PATH = os.path.join(PKG, "lib", f"_pw_torch.torch-{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}")
 HEADER = os.path.join(ROOT, "include", "pw_cuda.h")
 
 _lib = None

@@ -5,7 +5,8 @@ csrc/*.cpp (checkpoint ingestion) with the same driver (`-gencode
 arch=compute_100a,code=sm_100a -lineinfo`, no fast-math: the quantizer and the
 staged SwiGLU rely on IEEE division and rounding) and links
 mimo_prismwing_b200/lib/libpw_cuda.so in-tree, and compiles the binding for torch
-tensors (binding/pw_torch.cpp) to mimo_prismwing_b200/lib/_pw_torch.so with g++.
+tensors (binding/pw_torch.cpp) with g++ to mimo_prismwing_b200/lib/, one file per
+version of torch and Python.
 Objects go to mimo_prismwing_b200/_build/ (not committed).
 """
 from __future__ import annotations
@@ -18,12 +19,13 @@ import subprocess
 import sys
 import sysconfig
 
+from ._lib import BINDING_PATH
+
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "lib", "libpw_cuda.so")
-BINDING = os.path.join(PKG, "lib", "_pw_torch.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I" + os.path.join(ROOT, "include"),
@@ -40,13 +42,13 @@ def _stale(target: str, deps: list[str]) -> bool:
 def build_binding(force: bool = False) -> None:
     """The Python extension over torch's and the library's headers."""
     src = os.path.join(PKG, "binding", "pw_torch.cpp")
-    if not force and not _stale(BINDING, [src] + glob.glob(os.path.join(ROOT, "include", "*.h"))):
+    if not force and not _stale(BINDING_PATH, [src] + glob.glob(os.path.join(ROOT, "include", "*.h"))):
         return
     torch = importlib.util.find_spec("torch").submodule_search_locations[0]
     include = [os.path.join(ROOT, "include"), os.path.join(torch, "include"),
                os.path.join(torch, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden"]
-    cmd += ["-I" + d for d in include] + [src, "-o", BINDING, "-L" + os.path.join(torch, "lib")]
+    cmd += ["-I" + d for d in include] + [src, "-o", BINDING_PATH, "-L" + os.path.join(torch, "lib")]
     res = subprocess.run(cmd + ["-ltorch_python", "-ltorch_cpu", "-lc10"], capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)

@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import warnings
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -200,9 +201,14 @@ class WideMoeRuntime:
         self._banks = []
         self._bank_refs = []
         self._init_args()
-        entry = [ctypes.cast(f, ctypes.c_void_p).value for f in
-                 (self._L.pw_add_rms_norm, self._L.pw_linear, self._L.pw_fp8_linear_codes)]
-        self._calls = _lib.binding().Calls(rt.value, device, *entry)
+        try:
+            calls = _lib.binding().Calls
+        except (RuntimeError, ImportError) as e:  # not built for this torch and Python: the calls below run without it
+            warnings.warn(f"short calls take longer on the host: {e}", RuntimeWarning, stacklevel=2)
+        else:
+            entry = [ctypes.cast(f, ctypes.c_void_p).value for f in
+                     (self._L.pw_add_rms_norm, self._L.pw_linear, self._L.pw_fp8_linear_codes)]
+            self._calls = calls(rt.value, device, *entry)
 
     # reference constructors (src/wide_metal_moe.rs:165-171)
     @classmethod
