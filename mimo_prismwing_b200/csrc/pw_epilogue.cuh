@@ -77,7 +77,8 @@ __device__ __forceinline__ float gelu(float v) {
   q = fmaf(q, t, 0.202661037f);
   q = fmaf(q, t, 0.2263343185f);
   q = fmaf(q, t, 0.2256406248f);
-  const float h = 0.5f * v * (exp2f(-0.72134752f * v * v) * (t * q));
+  // far right of zero the tail is 0 times a bounded factor, not times an infinite v
+  const float h = 0.5f * fminf(v, 64.0f) * (exp2f(-0.72134752f * v * v) * (t * q));
   return v < 0.0f ? h : v - h;
 }
 __device__ __forceinline__ float activate(float v, uint32_t act) {

@@ -1,0 +1,41 @@
+"""The linear operators where their arithmetic ends: infinities, the activations' tails and long sums.
+
+Tolerances, derived before the first run.  One f32 operation is off by at most 2^-24 relative, expf and
+__fdividef by 2 ulps (2^-22), and below f32's smallest normal value by whole steps of 2^-149.  A tensor core
+adds 16 products to its accumulator with an error of at most 2^-23 of the sum, so sums of one sign in
+segments of 512 columns are within 32 * 2^-23, and every f32 addition that joins them adds 2^-24.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def rt():
+    from mimo_prismwing_b200.runtime import WideMoeRuntime
+    r = WideMoeRuntime.compile_with_fused_gate_up(0)
+    r.set_stream(torch.cuda.current_stream())
+    yield r
+    r.close()
+
+
+def of_bias(rt, values, act, width=1):
+    """The activation of these f32 values: zero products, the values as the bias."""
+    x = torch.zeros((width, 64), dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros((values.numel(), 64), dtype=torch.bfloat16, device="cuda")
+    got = rt.linear(x, w, bias=values, activation=act, out_dtype=torch.float32, asynchronous=True).output
+    torch.cuda.synchronize()
+    return got
+
+
+@pytest.mark.parametrize("width", [1, 40])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+def test_an_infinite_sum_stays_infinite(rt, act, width):
+    # from 25 on every activation is the value itself, to f32, and far below zero it is zero
+    v = torch.tensor([25.0, math.inf, 3.4e38, 1e19, 0.0, -1e19, -3.4e38], device="cuda")
+    got = of_bias(rt, v, act, width)
+    assert torch.equal(got, (v if act == "none" else v.clamp_min(0)).expand(width, -1))
+    assert rt.error_flags() & 32  # an infinity is reported
