@@ -56,7 +56,9 @@ __device__ __forceinline__ bool store_elem(void *p, uint64_t i, uint32_t dtype, 
 
 // The activations from their formulas, to a few ulps of f32 (__fdividef: 2),
 // without branches, so that the compiler interleaves several values.
-// exp(-v) overflows to infinity for v < -88 and the quotient is then -0, the limit.
+// The logistic function by exp of the negative magnitude, so that neither it nor the
+// divisor (1 to 2) leaves f32's range and the tail keeps its digits:
+// v / (1 + exp(-u)) = v exp(u) / (1 + exp(u)), the latter for u < 0.
 //
 // GELU: v (1 + erf(v / sqrt 2)) / 2 cancels below v ~ -4, so with z = |v| / sqrt 2
 // it is h = v erfc(z) / 2 for v < 0 and v - h for v > 0.  erfc(z) = exp(-z^2) t Q(t),
@@ -81,16 +83,18 @@ __device__ __forceinline__ float gelu(float v) {
   const float h = 0.5f * fminf(v, 64.0f) * (exp2f(-0.72134752f * v * v) * (t * q));
   return v < 0.0f ? h : v - h;
 }
+// v / (1 + exp(-u)) for a u of v's sign.
+__device__ __forceinline__ float gated(float v, float u) {
+  const float e = expf(-fabsf(u));
+  return __fdividef(u < 0.0f ? v * e : v, 1.0f + e);
+}
 __device__ __forceinline__ float activate(float v, uint32_t act) {
   switch (act) {
     case PW_ACT_RELU: return v < 0.0f ? 0.0f : v;  // a NaN stays a NaN
     case PW_ACT_GELU: return gelu(v);
-    case PW_ACT_GELU_TANH: {
-      // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
-      const float u = 1.5957691216057308f * fmaf(0.044715f * v * v, v, v);
-      return __fdividef(v, 1.0f + expf(-u));
-    }
-    case PW_ACT_SILU: return __fdividef(v, 1.0f + expf(-v));
+    // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
+    case PW_ACT_GELU_TANH: return gated(v, 1.5957691216057308f * fmaf(0.044715f * v * v, v, v));
+    case PW_ACT_SILU: return gated(v, v);
     default: return v;
   }
 }

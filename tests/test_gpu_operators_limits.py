@@ -39,3 +39,25 @@ def test_an_infinite_sum_stays_infinite(rt, act, width):
     got = of_bias(rt, v, act, width)
     assert torch.equal(got, (v if act == "none" else v.clamp_min(0)).expand(width, -1))
     assert rt.error_flags() & 32  # an infinity is reported
+
+
+@pytest.mark.parametrize("act,low,high", [("silu", -110.0, -60.0), ("gelu_tanh", -11.0, -8.0), ("gelu", -15.0, -10.0)])
+def test_activation_tails_keep_their_digits(rt, act, low, high):
+    v = torch.linspace(low, high, 4001, device="cuda")
+    d = v.double()
+    if act == "silu":
+        ref, rel = d * torch.exp(d) / (1 + torch.exp(d)), torch.zeros_like(d)
+    elif act == "gelu_tanh":
+        # the exponent is six f32 roundings from the value: |u| times their relative error
+        u = 2 * math.sqrt(2 / math.pi) * (d + 0.044715 * d ** 3)
+        ref, rel = d * torch.exp(u) / (1 + torch.exp(u)), u.abs() * 6 * 2.0 ** -24
+    else:
+        # the exponent is -v^2 log2(e) / 2 after three roundings, constant included; the polynomial is 6.6e-8 off
+        # and takes eleven roundings in its last steps' size
+        ref, rel = 0.5 * d * torch.erfc(-d / math.sqrt(2)), d * d / 2 * 3 * 2.0 ** -24 + 12 * 2.0 ** -24 + 1e-7
+    # exp, a product, a quotient, and the sum below it; then whole steps, which the value multiplies
+    bound = (rel + 6 * 2.0 ** -23) * ref.abs() + (2 * d.abs() + 4) * 2.0 ** -149
+    got = of_bias(rt, v, act)[0].double()
+    over = (got - ref).abs() - bound
+    at = int(over.argmax())
+    assert over.max().item() <= 0, f"{act} of {v[at].item()}: {got[at].item()}, not {ref[at].item()}"
