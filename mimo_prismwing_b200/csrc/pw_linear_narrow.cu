@@ -158,13 +158,25 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2)
                                : load_tail(xr[n], c, a.cols);
       }
     }
+    // Each group's products get accumulators of their own, added in f32: the MMA truncates
+    // when it adds to one (2400 rows x 65536 columns of one sign: 3.1e-5 off in one per
+    // warp).
+    float d[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[n][i] = 0.0f;
 #pragma unroll
     for (uint32_t j = 0; j < kDeep; ++j)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        mma16<BF16>(acc[n], wa[j].x, wb[j].x, wa[j].y, wb[j].y, xv[j][n].x, xv[j][n].y);
-        mma16<BF16>(acc[n], wa[j].z, wb[j].z, wa[j].w, wb[j].w, xv[j][n].z, xv[j][n].w);
+        mma16<BF16>(d[n], wa[j].x, wb[j].x, wa[j].y, wb[j].y, xv[j][n].x, xv[j][n].y);
+        mma16<BF16>(d[n], wa[j].z, wb[j].z, wa[j].w, wb[j].w, xv[j][n].z, xv[j][n].w);
       }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][i] += d[n][i];
   }
   pdl_launch_dependents();
 

@@ -22,6 +22,11 @@ def rt():
     r.close()
 
 
+def uniform(shape, seed, dtype, low, high):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.empty(shape, device="cuda").uniform_(low, high, generator=g).to(dtype)
+
+
 def of_bias(rt, values, act, width=1):
     """The activation of these f32 values: zero products, the values as the bias."""
     x = torch.zeros((width, 64), dtype=torch.bfloat16, device="cuda")
@@ -61,3 +66,23 @@ def test_activation_tails_keep_their_digits(rt, act, low, high):
     over = (got - ref).abs() - bound
     at = int(over.argmax())
     assert over.max().item() <= 0, f"{act} of {v[at].item()}: {got[at].item()}, not {ref[at].item()}"
+
+
+def long_product(x, w):
+    """x W^T in 64 bits, in pieces of the columns."""
+    got = torch.zeros((x.shape[0], w.shape[0]), dtype=torch.float64, device="cuda")
+    for k in range(0, x.shape[1], 1 << 16):
+        got += x[:, k:k + (1 << 16)].double() @ w[:, k:k + (1 << 16)].double().t()
+    return got
+
+
+@pytest.mark.parametrize("width", [1, 8, 9, 16])
+@pytest.mark.parametrize("rows,cols", [(8, 1 << 20), (2400, 65536), (600, 16384 + 8), (40, 8192)])
+def test_long_f32_sums_of_few_tokens_keep_their_digits(rt, width, rows, cols):
+    # sums of one sign: nothing cancels, so the error of the sum is the output's
+    x, w = uniform((width, cols), 1, torch.bfloat16, 0.5, 1.0), uniform((rows, cols), 2, torch.bfloat16, 0.5, 1.0)
+    ref = long_product(x, w)
+    got = rt.linear(x, w, out_dtype=torch.float32).output.double()
+    # eight warps at least share the columns; joining them and up to eight splits is 16 additions
+    bound = 32 * 2.0 ** -23 + (cols / 512 / 8 + 16) * 2.0 ** -24
+    assert ((got - ref).abs() / ref).max().item() <= bound
