@@ -14,12 +14,12 @@
 //    so the shared memory that a tensor core reads per product is half of what a
 //    128 x 256 tile of one CTA needs.  Persistent pairs, two accumulators, all of
 //    a tile's K in one accumulator.  Bound by the tensor pipe.
-//  * k_linear_tile, for the widths between and for f32 outputs: 128 x 32, 64 or
-//    128 tiles of one CTA.  K runs in segments of 512 columns: each gets a fresh
-//    accumulator, and the epilogue adds the segments in registers.  (The tensor
-//    pipe truncates when it adds to an accumulator: over 4096 columns in one
-//    accumulator an f32 result was 4.4e-6 off, with segments it is below 1e-6; a
-//    16-bit result does not show it.)
+//  * k_linear_tile, for the widths between and for what a pair's accumulator would not
+//    hold exactly enough (f32 outputs, long K): 128 x 32, 64 or 128 tiles of one CTA.
+//    K runs in segments of 512 columns: each gets a fresh accumulator, and the epilogue
+//    adds the segments in registers.  (The tensor pipe truncates when it adds to an
+//    accumulator: over 4096 columns in one accumulator an f32 result was 4.4e-6 off,
+//    with segments it is below 1e-6; a 16-bit result does not show it.)
 //
 // When the tiles are fewer than the SMs, the CTAs (pairs) of a cluster split K:
 // HBM bounds these widths, and a stream over a third of the SMs does not reach
@@ -720,7 +720,11 @@ cudaError_t launch_linear(const LinearArgs &a, int num_sms, cudaStream_t stream)
   // 16384 rows 30.0 against 25.1 us).
   if (a.width <= 8u || (a.width <= 16u && a.rows <= 16u * (uint32_t)num_sms))
     return launch_linear_narrow(a, num_sms, stream);
-  if (a.ep.y_dtype != PW_DTYPE_F32 && a.width > 128u) return lin::launch_pair(a, num_sms, stream);
+  // A pair's accumulator takes all of K, in K / 16 additions that truncate by up to 2^-23:
+  // within a quarter of the output's half step (bf16 2^-8, f16 2^-11) for these K.  The
+  // tile's segments cost time (2048 x 4096 x 16384: pairs 201 us, tiles 300 us).
+  const uint32_t pair_cols = a.ep.y_dtype == PW_DTYPE_BF16 ? 131072u : a.ep.y_dtype == PW_DTYPE_F16 ? 16384u : 0u;
+  if (a.cols <= pair_cols && a.width > 128u) return lin::launch_pair(a, num_sms, stream);
   if (a.width <= 32u) return lin::launch_tile<32>(a, num_sms, stream);
   if (a.width <= 64u) return lin::launch_tile<64>(a, num_sms, stream);
   return lin::launch_tile<128>(a, num_sms, stream);

@@ -86,3 +86,14 @@ def test_long_f32_sums_of_few_tokens_keep_their_digits(rt, width, rows, cols):
     # eight warps at least share the columns; joining them and up to eight splits is 16 additions
     bound = 32 * 2.0 ** -23 + (cols / 512 / 8 + 16) * 2.0 ** -24
     assert ((got - ref).abs() / ref).max().item() <= bound
+
+
+@pytest.mark.parametrize("dtype,cols", [("f16", 1 << 18), ("f16", 16384), ("bf16", 1 << 19), ("bf16", 131072)])
+def test_long_16_bit_sums_of_many_tokens_keep_their_digits(rt, dtype, cols):
+    # off by the one rounding and by a quarter of it at most
+    t = {"f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    x, w = uniform((136, cols), 3, t, 0.5, 1.0), uniform((136, cols), 4, t, 2.0 ** -6, 2.0 ** -5)
+    ref = long_product(x, w)
+    got = rt.linear(x, w).output.double()
+    half = torch.finfo(t).eps / 2
+    assert ((got - ref).abs() / ref).max().item() <= half * 1.25
