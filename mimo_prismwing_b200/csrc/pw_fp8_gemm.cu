@@ -51,12 +51,14 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint32_t kSmemLimit = 227u * 1024u;
 constexpr uint32_t kMaxBlocks = 32;   // K <= 4096
-// Measured cycles (B200 at 1.9 GHz): the one-CTA tile 640 per block and 5500 per wave, a
-// pair's, of four times the products, 950 and 11000; joining K splits costs 13500 and
-// 28000 in place of the latter.  In us, one CTA / pair: 512 x 4096 x 4096 15.0 / 22.9, 768 x
+// Measured cycles (B200 at 1.9 GHz): the one-CTA tile 640 per block and 5500 per wave,
+// 13500 where K splits are joined; a pair's, of four times the products, 950 and 11000.
+// (Pairs do not split K: joining took them 28000, and wherever that beat an unsplit pair,
+// split one-CTA tiles beat both.)  In us, one CTA / pair: 512 x 4096 x 4096 15.0 / 22.9, 768 x
 // 4096 x 4096 27.9 / 23.9, 384 x 13568 x 4096 41.0 / 43.8, 1024 x 13568 x 4096 83.6 / 65.4;
 // unsplit / split one-CTA tiles: 203 x 4096 x 2048 9.6 / 10.8, 64 x 4096 x 4096 14.4 / 9.9.
-constexpr TileCost kCostOne{640u, 5500u, 13500u}, kCostPair{950u, 11000u, 28000u};
+constexpr TileCost kCostOne{640u, 5500u, 13500u};
+constexpr uint64_t kPairBlock = 950u, kPairWave = 11000u;
 constexpr uint32_t kTokenGroup = 8;   // token tiles that neighbouring pairs share weights over
 // Register split: 256 x 240 + 128 x 24, all of the 384 x 168 at launch.
 constexpr int kRegsLaunch = 168, kRegsEpi = 240, kRegsOther = 24;
@@ -86,7 +88,7 @@ struct Cfg {
   static constexpr uint32_t TMEM_COLS = NACC * BN;
   static_assert(SMEM <= kSmemLimit, "shared memory");
   // the ring and, behind it, the boxes, which K splits do not use
-  static_assert((BN + 8u * kMaxSplits) * kTileRows * 4u <= XS, "exchange buffer");
+  static_assert(PAIR || (BN + 8u * kMaxSplits) * kTileRows * 4u <= XS, "exchange buffer");
 };
 
 struct Args {
@@ -156,9 +158,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
   sh.abort = reinterpret_cast<volatile int *>(smem + C::MISC + 4);
 
   const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
-  // PAIR: cluster CTAs 2 k and 2 k + 1 are the pair of K split k; else CTA k is split k
-  const uint32_t splits = A.splits, cta = PAIR || splits > 1u ? cluster_rank() : 0u;
-  const uint32_t rank = PAIR ? cta & 1u : 0u, lead = PAIR ? cta & ~1u : cta, split = PAIR ? cta / 2u : cta;
+  // a cluster is a pair, or the CTAs that split a tile's K
+  const uint32_t splits = PAIR || RES ? 1u : A.splits, cta = PAIR || splits > 1u ? cluster_rank() : 0u;
+  const uint32_t rank = PAIR ? cta : 0u, lead = PAIR ? 0u : cta, split = PAIR ? 0u : cta;
   constexpr uint32_t CTAS = PAIR ? 2u : 1u;
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < NST; ++i) {
@@ -274,8 +276,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
 #pragma unroll
             for (uint32_t s = 0; s < 4; ++s) mma_f8<PAIR>(d, ad + 2u * s, bd + 2u * s, idesc, s ? 1u : 0u);
           }
-          mma_commit<PAIR>(&sh.tfull[acc], 3u << lead);
-          mma_commit<PAIR>(&sh.empty[slot], 3u << lead);
+          mma_commit<PAIR>(&sh.tfull[acc], 3u);
+          mma_commit<PAIR>(&sh.empty[slot], 3u);
           pending |= 1u << acc;
           pend_parity = (pend_parity & ~(1u << acc)) | (aphase << acc);
           if (++acc == NACC) {
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
       }
       tc::cp_async_commit();
     };
-    const uint32_t tempty_lead = map_rank(smem_addr(sh.tempty), cta & ~(CTAS - 1u));  // the leading CTA's
+    const uint32_t tempty_lead = map_rank(smem_addr(sh.tempty), lead);
     const bool quad_r = quad_access(a.ep.residual, a.ep.residual_stride, a.ep.residual_dtype);
     const bool quad_y = quad_access(a.ep.y, a.ep.y_stride, a.ep.y_dtype);
     // this warp's output boxes: 32 tokens x 64 bytes, `box` counts them over all tiles
@@ -456,8 +458,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         }
       }
 
-      if (!RES && splits > 1u) {
-        const Exchange x(sh.ring, splits, split, CTAS, rank, min(BN, a.rows - rt * BN));
+      if (!PAIR && !RES && splits > 1u) {
+        const Exchange x(sh.ring, splits, split, 1u, 0u, min(BN, a.rows - rt * BN));
         __syncwarp();
         cluster_sync_all();  // every CTA's MMAs have read their last stage
         if (active) {
@@ -662,16 +664,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
   }
 }
 
-// Tiles, column blocks and the best K split of a kernel on these sizes.
+// Tiles, column blocks, and the best K split of one-CTA tiles on these sizes.
 template <bool PAIR>
 Splits plan(const Fp8CodesArgs &a, int num_sms, uint32_t &row_tiles, uint32_t &token_tiles, uint32_t &stages) {
   using C = Cfg<PAIR, false>;
-  constexpr uint32_t CTAS = PAIR ? 2u : 1u, kTokens = CTAS * kTileRows;
+  constexpr uint32_t kTokens = (PAIR ? 2u : 1u) * kTileRows;
   row_tiles = (a.rows + C::BN - 1u) / C::BN;
   token_tiles = (a.width + kTokens - 1u) / kTokens;
   stages = a.K / 128u;
-  return best_splits<k_fp8_gemm<PAIR, false>>(PAIR ? kCostPair : kCostOne, (uint64_t)row_tiles * token_tiles, stages,
-                                              kMaxSplits / CTAS, CTAS, kThreads, C::SMEM, num_sms);
+  const uint64_t tiles = (uint64_t)row_tiles * token_tiles;
+  if constexpr (PAIR) {
+    const uint64_t pairs = (uint64_t)num_sms / 2u;
+    return {1u, (tiles + pairs - 1u) / pairs * (stages * kPairBlock + kPairWave)};
+  } else {
+    return best_splits<k_fp8_gemm<false, false>>(kCostOne, tiles, stages, kMaxSplits, 1u, kThreads, C::SMEM, num_sms);
+  }
 }
 
 // Raises the kernel's shared-memory limit, without which its occupancy is none.
@@ -733,8 +740,8 @@ cudaError_t launch_one(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream) 
 cudaError_t launch_fp8_gemm(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream) {
   using namespace fp8g;
   if (a.width == 0 || a.rows % 64u || a.K == 0 || a.K % 128u || a.K > 128u * kMaxBlocks) return cudaErrorInvalidValue;
-  cudaError_t e;
-  if ((e = prepare<false, false>()) != cudaSuccess || (e = prepare<true, false>()) != cudaSuccess) return e;
+  const cudaError_t e = prepare<false, false>();
+  if (e != cudaSuccess) return e;
   uint32_t r, t, s;
   if (a.width <= 128u || plan<false>(a, num_sms, r, t, s).cost <= plan<true>(a, num_sms, r, t, s).cost)
     return launch_one<false>(a, num_sms, stream);
