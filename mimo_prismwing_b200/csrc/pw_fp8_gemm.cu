@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_fp8_gemm(const __grid_constant_
         const uint32_t first = x.split * x.share, mid = x.share / 2u & ~7u;
         const uint32_t in_tile = first < x.cols ? min(x.share, x.cols - first) : 0u;
         // this thread's token, columns [begin, end) of the share, eight at a time
-        // (rows are a multiple of 64), their residual and bias one step ahead
+        // (rows are a multiple of 128), their residual and bias one step ahead
         const uint32_t begin = half ? mid : 0u, end = half ? in_tile : min(mid, in_tile);
         const bool mine = tok_q + lane < a.width;
         Quads<2, false> g{tok_q + lane, rt * BN + first + begin, 0u};
@@ -739,7 +739,9 @@ cudaError_t launch_one(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream) 
 
 cudaError_t launch_fp8_gemm(const Fp8CodesArgs &a, int num_sms, cudaStream_t stream) {
   using namespace fp8g;
-  if (a.width == 0 || a.rows % 64u || a.K == 0 || a.K % 128u || a.K > 128u * kMaxBlocks) return cudaErrorInvalidValue;
+  // a warp of the pair's epilogue takes 128 output columns whole
+  if (a.width == 0 || a.rows == 0 || a.rows % 128u || a.K == 0 || a.K % 128u || a.K > 128u * kMaxBlocks)
+    return cudaErrorInvalidValue;
   const cudaError_t e = prepare<false, false>();
   if (e != cudaSuccess) return e;
   uint32_t r, t, s;
