@@ -447,8 +447,9 @@ cudaError_t launch_shape(const AddNormArgs &a, uint32_t steps, uint32_t threads,
   if (steps == 2u) return launch_one<T, VEC, 2, false>(a, threads, num_sms, stream);
   // Fewer registers make more CTAs resident, and a turn of each slower: worth it when
   // the rows then take fewer turns (bf16 with residual and codes, usual / slim: 2048 x
-  // 4096, 4 / 3 turns, 15.8 / 14.4 us; 16384 x 1024, 7 / 6 turns, 23.9 / 23.0 us; 2048 x
-  // 2048, 2 turns both, 7.0 / 7.7 us; f32 rows leave slim CTAs no ring: 35.7 / 39.2 us).
+  // 4096, 4 / 3 turns, 14.7 / 13.8 us; 16384 x 1024, 7 / 6 turns, 23.9 / 22.5 us; 2048 x
+  // 2048, 2 turns both, 7.3 / 8.0 us; f32 rows leave slim CTAs no ring: 2048 x 4096 20.4 /
+  // 22.9 us).
   if constexpr (VEC != kElements && sizeof(T) == 2) {
     if (threads <= kSlimThreads) {
       const uint32_t usual = resident<k_add_norm<T, VEC, 4, false>>(threads) * (uint32_t)num_sms;

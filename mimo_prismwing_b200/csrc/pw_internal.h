@@ -275,11 +275,13 @@ cudaError_t launch_linear_narrow(const LinearArgs &a, int num_sms, cudaStream_t 
 // converted from x_dtype.
 cudaError_t launch_convert_rows(const void *x, uint64_t x_stride, uint32_t x_dtype, uint32_t rows, uint32_t cols,
                                 void *out, uint64_t out_stride, uint32_t dtype, cudaStream_t stream);
-// cuTensorMapEncodeTiled over 16-bit rows: with k_blocks, the view {64
-// columns, rows, cols / 64} in boxes {64, box_rows, k_blocks}; without, the
-// view {cols, rows, 1} in boxes {64, box_rows, 1}, zero past the last column.
+// cuTensorMapEncodeTiled over output rows (or a residual's) of any PW_DTYPE_*, in
+// boxes of 64 bytes x box_rows.
 bool encode_out_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride, uint32_t dtype,
                     uint32_t box_rows);
+// The same over 16-bit rows to load: with k_blocks, the view {64 columns, rows,
+// cols / 64} in boxes {64, box_rows, k_blocks}; without, the view {cols, rows, 1}
+// in boxes {64, box_rows, 1}, zero past the last column.
 bool encode_rows16_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride,
                        uint32_t dtype, uint32_t box_rows, uint32_t k_blocks);
 

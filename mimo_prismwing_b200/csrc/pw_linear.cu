@@ -725,6 +725,16 @@ cudaError_t launch_linear(const LinearArgs &a, int num_sms, cudaStream_t stream)
   // tile's segments cost time (2048 x 4096 x 16384: pairs 201 us, tiles 300 us).
   const uint32_t pair_cols = a.ep.y_dtype == PW_DTYPE_BF16 ? 131072u : a.ep.y_dtype == PW_DTYPE_F16 ? 16384u : 0u;
   if (a.cols <= pair_cols && a.width > 128u) return lin::launch_pair(a, num_sms, stream);
+  // Below and above, the token count chooses: a wide tile reads the weights for fewer
+  // column tiles, a narrow one pads less.  us at 32 / 64 / 128 / pair, bf16:
+  //    32 tokens  [4096, 4096]  9.3 /  9.4 / 10.6 / 13.7   [16384, 4096] 26.2 / 26.7 / 28.4 / 28.9
+  //    64         [4096, 8192] 17.5 / 16.0 / 17.4 / 20.7   [16384, 4096] 29.8 / 27.2 / 29.8 / 30.2
+  //   128         [4096, 8192] 26.2 / 19.5 / 19.2 / 22.6   [16384, 4096] 48.0 / 32.7 / 30.7 / 32.7
+  //   200         [4096, 8192] 47.0 / 28.5 / 24.9 / 24.7
+  //   256         [4096, 4096] 26.5 / 16.8 / 16.6 / 19.6   [16384, 4096] 79.8 / 53.3 / 42.0 / 34.4
+  //   512         [4096, 8192] 89.4 / 51.3 / 38.8 / 32.9
+  // Where the tiles are few it is not always the best: 256 tokens of [4096, 4096] above, and
+  // 100 of them 15.6 / 12.7 / 13.6 / 15.6.
   if (a.width <= 32u) return lin::launch_tile<32>(a, num_sms, stream);
   if (a.width <= 64u) return lin::launch_tile<64>(a, num_sms, stream);
   return lin::launch_tile<128>(a, num_sms, stream);

@@ -66,8 +66,7 @@ bool encode_act_maps(CUtensorMap (&out)[4], const void *base, uint32_t rows, uin
   return true;
 }
 
-// 16-bit rows for the linear layer's TMA loads (zero past every end).
-// Output rows as boxes of 64 bytes x box_rows, 64B-swizzled.
+// Output rows, and the residual that joins them, as boxes of 64 bytes x box_rows, 64B-swizzled.
 bool encode_out_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride, uint32_t dtype,
                     uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
@@ -86,6 +85,7 @@ bool encode_out_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t 
          CUDA_SUCCESS;
 }
 
+// 16-bit rows for the linear layer's TMA loads (zero past every end).
 bool encode_rows16_map(CUtensorMap *out, const void *base, uint32_t rows, uint32_t cols, uint64_t stride,
                        uint32_t dtype, uint32_t box_rows, uint32_t k_blocks) {
   EncodeTiledFn fn = encode_fn();

@@ -427,10 +427,11 @@ class WideMoeRuntime:
     # ------------------------------------- residual, norm, linear layers
     # These calls take a few microseconds on the device for a single token, so
     # their host side is kept short.  An asynchronous call on device tensors goes
-    # through the compiled binding (one token's linear layer 4.5 us on the host, 9.5
-    # without; the norm with all its outputs 7.5 and 14.5); what that does not take (None) comes here: one check per tensor,
-    # and the descriptors (the structures above) packed at once into a block that the
-    # runtime keeps (like the runtime's other state, it serves one call at a time).
+    # through the compiled binding where there is one (one token's linear layer 4.5 us on
+    # the host, 9.5 without; the norm with all its outputs 7.5 and 14.5); what that does
+    # not take (None) comes here: one check per tensor, and the descriptors (the
+    # structures above) packed at once into a block that the runtime keeps (like the
+    # runtime's other state, it serves one call at a time).
     _calls = None
     _NORM_ARGS = struct.Struct("=QIIf4x" + "QQII" * 4)       # Norm, then Rows of x, residual, sum, y
     _LINEAR_ARGS = struct.Struct("=QQIIII" + "QQII" + "QIIQQII" + "QQII")  # Dense, Rows of x, Epilogue, Rows of y
