@@ -1245,10 +1245,12 @@ int pw_linear(pw_runtime *rt, const pw_dense *w, const pw_rows *x, uint32_t widt
     {
       ProfScope ps(rt, P_PROJ, 1);
       PdlScope pdl(!rt->profiling);
-      CK(launch_linear(a, rt->num_sms, rt->stream));
+      const cudaError_t launched = launch_linear(a, rt->num_sms, rt->stream);
+      // behind the copy even where nothing reads it
+      if (convert && !call.host() && !captured) CK(cudaEventRecord(rt->convert_done, rt->stream));
+      CK(launched);
     }
     if (captured) CK(graph.give());
-    else if (convert && !call.host()) CK(cudaEventRecord(rt->convert_done, rt->stream));
     if (call.host()) CK(copy_rows(yr, dy, width, N, cudaMemcpyDeviceToHost, rt->stream));
   }
   return call.finish((uint64_t)N * K * 2u);
